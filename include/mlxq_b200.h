@@ -385,6 +385,74 @@ int mlxq_decode_advance(int32_t* positions, int32_t* kv_lens, int32_t* slots,
                         const int32_t* block_table, int64_t max_blocks, int64_t batch,
                         int page_size, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * A paged KV cache held in 16, 8 or 4 bits. One layer's pools: keys and values
+ * [num_pages * page_size, n_kv_heads, head_dim] of dtype (bits 16), or packed codes
+ * [rows, n_kv_heads, head_dim * bits / 32] uint32 with scales and biases
+ * [rows, n_kv_heads, head_dim / group_size] of dtype (bits 8 or 4), each head's row laid
+ * out as mlxq_quantize lays out a row. A code q stands for scale * q + bias rounded once
+ * to dtype, in every operator below. head_dim 64 or 128; page_size 8, 16 or 32;
+ * group_size 32, 64 or 128, at most head_dim; pointers 16-byte aligned (k, v) and
+ * 4-byte aligned (scales, biases). The struct is read during the call.
+ */
+typedef struct mlxq_kv_cache {
+    void* k;
+    void* v;
+    void* k_scales; /* NULL with bits 16, as are the next three */
+    void* k_biases;
+    void* v_scales;
+    void* v_biases;
+    int64_t num_pages;
+    int32_t page_size, n_kv_heads, head_dim, bits, group_size, dtype;
+} mlxq_kv_cache;
+
+/*
+ * Per-head RMSNorm, rotation and the append, in one launch: what mlxq_rope_kv_append does
+ * with, before the rotation, each query head h normalised as
+ * h * rsqrt(mean(h^2) + eps) * q_norm and each key head with k_norm (head_dim weights of
+ * dtype; NULL leaves that side as it is): the head norms of Qwen3-style attention
+ * (models/qwen3.py of the reference). Norm and rotation are one 32-bit
+ * computation rounded once; the angle is reduced in 64 bits. With bits 8 or 4 the rounded
+ * rows are quantized as mlxq_quantize would quantize them. Slots outside
+ * [0, num_pages * page_size) are skipped; two tokens of one call must not share a slot.
+ */
+int mlxq_norm_rope_kv_append(const mlxq_kv_cache* cache, const void* qkv, int64_t ld, void* q_out,
+                             const void* q_norm, const void* k_norm, float eps,
+                             const int32_t* positions, const int32_t* slots, int64_t tokens,
+                             int n_q_heads, float rope_base, void* stream);
+
+/*
+ * The values of cache rows slots[0..n): k_out, v_out [n, n_kv_heads, head_dim] of dtype;
+ * slots outside the pool give zero rows.
+ */
+int mlxq_kv_cache_read(const mlxq_kv_cache* cache, const int32_t* slots, int64_t n, void* k_out,
+                       void* v_out, void* stream);
+
+/*
+ * Paged attention for several query rows per sequence (mlxq_paged_attention_decode and
+ * _prefill's operator over a cache of any width, and trees of drafted tokens). Sequence b
+ * of `batch` owns rows [cu_q[b], cu_q[b+1]) of q and out [total, n_q_heads, head_dim], at
+ * most max_q_len of them; cu_q NULL: row b alone (total = batch, max_q_len = 1). Its
+ * kv_lens[b] <= max_kv_len cached keys include those n new tokens, at the last n positions.
+ * New token i sees every key before them and, of the new ones,
+ *   tree_mask NULL: those up to itself (causal);
+ *   tree_mask [total] int64: new token j where bit j of its own word is set (max_q_len at
+ *   most 64; bits of its ancestors and of itself, for a tree).
+ * A row that sees no key is zero, and so are the rows of out behind cu_q[batch]. Keys on
+ * a page id outside [0, num_pages) are left out. A value that is not finite reaches the
+ * rows that do not see its key only where the key is one of the sequence's own new tokens.
+ * n_q_heads / n_kv_heads <= 8. The workspace (mlxq_paged_attention_rows_workspace_size bytes, 256-byte aligned,
+ * contents arbitrary) is used until the call's work on the stream has finished.
+ */
+size_t mlxq_paged_attention_rows_workspace_size(const mlxq_kv_cache* cache, int64_t batch,
+                                                int64_t max_q_len, int64_t max_kv_len,
+                                                int n_q_heads);
+int mlxq_paged_attention_rows(const mlxq_kv_cache* cache, const void* q, const int32_t* cu_q,
+                              int64_t total, int64_t max_q_len, const int32_t* block_table,
+                              int64_t max_blocks, const int32_t* kv_lens, int64_t max_kv_len,
+                              const int64_t* tree_mask, void* out, int64_t batch, int n_q_heads,
+                              float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,10 +50,25 @@ EXPORTED = (
     "mlxq_moe_sort",
     "mlxq_gather_swiglu_supported",
     "mlxq_gather_qmm_swiglu",
+    "mlxq_norm_rope_kv_append",
+    "mlxq_kv_cache_read",
+    "mlxq_paged_attention_rows_workspace_size",
+    "mlxq_paged_attention_rows",
 )
 
 _lock = threading.Lock()
 _lib = None
+
+
+class KVCache(ctypes.Structure):
+    """mlxq_kv_cache: one layer's pools of a paged cache in 16, 8 or 4 bits."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scales", ctypes.c_void_p), ("k_biases", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("v_biases", ctypes.c_void_p),
+                ("num_pages", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("bits", ctypes.c_int32), ("group_size", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
 
 
 class LibraryError(RuntimeError):
@@ -140,6 +155,17 @@ def load(path: str | None = None):
         L.mlxq_gather_qmm_swiglu.argtypes = [vp, vp, vp, vp, vp, i64, vp, vp, i64, i64, i64, i64,
                                              i64, i64, i32, i32, i32, i32, vp, sz, vp]
         L.mlxq_gather_qmm_swiglu.restype = i32
+        kvp = ctypes.POINTER(KVCache)
+        L.mlxq_norm_rope_kv_append.argtypes = [kvp, vp, i64, vp, vp, vp, f32, vp, vp, i64, i32,
+                                               f32, vp]
+        L.mlxq_norm_rope_kv_append.restype = i32
+        L.mlxq_kv_cache_read.argtypes = [kvp, vp, i64, vp, vp, vp]
+        L.mlxq_kv_cache_read.restype = i32
+        L.mlxq_paged_attention_rows_workspace_size.argtypes = [kvp, i64, i64, i64, i32]
+        L.mlxq_paged_attention_rows_workspace_size.restype = sz
+        L.mlxq_paged_attention_rows.argtypes = [kvp, vp, vp, i64, i64, vp, i64, vp, i64, vp, vp,
+                                                i64, i32, f32, vp, sz, vp]
+        L.mlxq_paged_attention_rows.restype = i32
         v = L.mlxq_abi_version()
         if v != ABI_VERSION:
             raise LibraryError(f"{p} has ABI version {v}, expected {ABI_VERSION}; rebuild it")

@@ -23,6 +23,7 @@ from . import _lib
 from .core import Workspace
 
 __all__ = ["rms_norm", "rope_kv_append", "paged_attention_decode", "paged_attention_prefill",
+           "paged_attention_tree", "tree_masks", "kv_cache_read", "QuantizedKV",
            "quantized_embedding", "decode_advance", "PagedKVCache", "PagedBatch"]
 
 _DT = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
@@ -40,6 +41,100 @@ def _stream(dev: torch.device):
 
 def _p(t):
     return None if t is None else t.data_ptr()
+
+
+@dataclass(frozen=True)
+class QuantizedKV:
+    """One layer's keys or values held in 8 or 4 bits: the pool a 16-bit cache tensor
+    [pages, page_size, n_kv_heads, head_dim] stands for, each head's row quantized as
+    quantize() does it. codes uint32 [pages, page_size, n_kv_heads, head_dim*bits/32],
+    scales and biases [pages, page_size, n_kv_heads, head_dim/group_size] of the
+    activation dtype; a code q stands for scale * q + bias, rounded once to that dtype.
+    Takes a cache tensor's place in rope_kv_append, kv_cache_read and the paged
+    attention functions (keys and values of the same width)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    biases: torch.Tensor
+    group_size: int = 64
+    bits: int = 4
+
+    def __post_init__(self):
+        if self.bits not in (4, 8):
+            raise ValueError(f"a quantized cache has 4 or 8 bits, got {self.bits}")
+        if self.group_size not in (32, 64, 128):
+            raise ValueError(f"group_size must be 32, 64 or 128, got {self.group_size}")
+        c, s, b = self.codes, self.scales, self.biases
+        if c.dtype not in (torch.uint32, torch.int32) or s.dtype not in _DT or b.dtype != s.dtype:
+            raise ValueError("codes must be uint32, scales and biases bfloat16 or float16")
+        if c.ndim != 4 or s.shape != b.shape or s.shape[:3] != c.shape[:3] or \
+                s.shape[3] * self.group_size * self.bits != c.shape[3] * 32:
+            raise ValueError("codes [pages, page_size, n_kv_heads, head_dim*bits/32] and scales, "
+                             "biases [..., head_dim/group_size] expected")
+        if not (c.is_contiguous() and s.is_contiguous() and b.is_contiguous()):
+            raise ValueError("a quantized cache's tensors must be contiguous")
+        if c.device != s.device or c.device != b.device:
+            raise ValueError("a quantized cache's tensors must be on one device")
+
+    @classmethod
+    def zeros(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+              group_size: int = 64, bits: int = 4, dtype=torch.bfloat16, device="cuda"):
+        """An empty pool."""
+        if group_size <= 0 or head_dim % group_size:
+            raise ValueError(f"head_dim {head_dim} is not a multiple of group_size {group_size}")
+        rows = (num_pages, page_size, n_kv_heads)
+        sb = [torch.zeros(*rows, head_dim // group_size, dtype=dtype, device=device)
+              for _ in range(2)]
+        return cls(torch.zeros(*rows, head_dim * bits // 32, dtype=torch.int32,
+                               device=device).view(torch.uint32), *sb, group_size, bits)
+
+    @property
+    def shape(self) -> tuple:
+        return (*self.codes.shape[:3], self.scales.shape[3] * self.group_size)
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.scales.dtype
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+
+def _kv_struct(k, v) -> _lib.KVCache:
+    """The C ABI's view of one layer's pools (16-bit tensors, or QuantizedKV)."""
+    if isinstance(k, QuantizedKV):
+        if not isinstance(v, QuantizedKV) or v.codes.shape != k.codes.shape or \
+                v.scales.shape != k.scales.shape or v.bits != k.bits or v.dtype != k.dtype:
+            raise ValueError("keys and values must share a quantized cache's shape and width")
+        pages, page, hkv = k.codes.shape[:3]
+        return _lib.KVCache(k.codes.data_ptr(), v.codes.data_ptr(), k.scales.data_ptr(),
+                            k.biases.data_ptr(), v.scales.data_ptr(), v.biases.data_ptr(), pages,
+                            page, hkv, k.scales.shape[3] * k.group_size, k.bits, k.group_size,
+                            _DT[k.dtype])
+    if isinstance(v, QuantizedKV) or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError("k_cache and v_cache must share shape and dtype")
+    if k.ndim != 4 or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError("caches must be contiguous [pages, page_size, n_kv_heads, head_dim]")
+    pages, page, hkv, hd = k.shape
+    return _lib.KVCache(k.data_ptr(), v.data_ptr(), None, None, None, None, pages, page, hkv, hd,
+                        16, 0, _code(k, "the cache"))
+
+
+def _on(dev: torch.device, *ts) -> None:
+    """Every tensor on the CUDA device `dev`."""
+    if dev.type != "cuda":
+        raise ValueError(f"expected CUDA tensors, got a tensor on {dev}")
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors are on different devices ({dev} and {t.device})")
+
+
+def _call(dev: torch.device, call):
+    """call(stream) with `dev` current, on its current stream."""
+    if torch.cuda.current_device() == dev.index:
+        return call(_stream(dev))
+    with torch.cuda.device(dev):
+        return call(_stream(dev))
 
 
 def _i32(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -75,13 +170,21 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
 
 
 def rope_kv_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
-                   k_cache: torch.Tensor, v_cache: torch.Tensor, n_heads: int, n_kv_heads: int,
-                   head_dim: int, base: float = 10000.0) -> torch.Tensor:
+                   k_cache, v_cache, n_heads: int, n_kv_heads: int,
+                   head_dim: int, base: float = 10000.0, q_norm: torch.Tensor | None = None,
+                   k_norm: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
     """RoPE of the queries and keys in `qkv` [T, (n_heads + 2 n_kv_heads) * head_dim]
     (the fused q/k/v projection's output) at `positions` [T], keys and values written
     to cache rows `slots` [T] (page * page_size + offset, -1 = skip) of
-    k_cache / v_cache [pages, page_size, n_kv_heads, head_dim]. Returns the rotated
-    queries [T, n_heads, head_dim]."""
+    k_cache / v_cache [pages, page_size, n_kv_heads, head_dim], or quantized into a pair
+    of QuantizedKV. With q_norm / k_norm [head_dim] each query / key head is RMS-normed
+    first (the head norms of Qwen3-style attention, models/qwen3.py of the reference),
+    in the same launch and with one rounding. Returns the rotated queries
+    [T, n_heads, head_dim]. Two tokens of a call must not share a slot."""
+    if q_norm is not None or k_norm is not None or isinstance(k_cache, QuantizedKV) or \
+            isinstance(v_cache, QuantizedKV):
+        return _norm_rope_append(qkv, positions, slots, k_cache, v_cache, n_heads, n_kv_heads,
+                                 head_dim, base, q_norm, k_norm, eps)
     dt = _code(qkv, "qkv")
     if qkv.ndim != 2 or qkv.stride(1) != 1:
         raise ValueError("qkv must be a 2-D tensor with contiguous rows")
@@ -103,6 +206,127 @@ def rope_kv_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tens
     return q
 
 
+def _norm_rope_append(qkv, positions, slots, k_cache, v_cache, n_heads, n_kv_heads, head_dim,
+                      base, q_norm, k_norm, eps):
+    kv = _kv_struct(k_cache, v_cache)
+    if qkv.ndim != 2 or qkv.stride(1) != 1 or qkv.dtype != k_cache.dtype:
+        raise ValueError("qkv must be a 2-D tensor with contiguous rows, of the caches' dtype")
+    if kv.n_kv_heads != n_kv_heads or kv.head_dim != head_dim:
+        raise ValueError("caches must hold n_kv_heads heads of head_dim")
+    T = qkv.shape[0]
+    if n_heads <= 0 or qkv.shape[1] < (n_heads + 2 * n_kv_heads) * head_dim:
+        raise ValueError("qkv's rows must hold q, k and v")
+    for w in (q_norm, k_norm):
+        if w is not None and (w.shape != (head_dim,) or w.dtype != qkv.dtype or
+                              not w.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous [{head_dim}] of dtype {qkv.dtype}")
+    positions, slots = _i32(positions, "positions"), _i32(slots, "slots")
+    if positions.shape != (T,) or slots.shape != (T,):
+        raise ValueError(f"positions and slots must be [{T}]")
+    dev = qkv.device
+    _on(dev, positions, slots, k_cache, v_cache, q_norm, k_norm)
+    q = torch.empty(T, n_heads, head_dim, dtype=qkv.dtype, device=dev)
+    # (a single row's stride is arbitrary)
+    ld = qkv.stride(0) if T > 1 else (qkv.shape[1] + 7) // 8 * 8
+    rc = _call(dev, lambda st: _lib.load().mlxq_norm_rope_kv_append(
+        kv, _p(qkv), ld, _p(q), _p(q_norm), _p(k_norm), float(eps), _p(positions), _p(slots), T,
+        n_heads, float(base), st))
+    _lib.check(rc, "rope_kv_append")
+    return q
+
+
+def kv_cache_read(k_cache, v_cache, slots: torch.Tensor):
+    """The values cache rows `slots` [n] (page * page_size + offset) hold: keys and values
+    [n, n_kv_heads, head_dim] in the cache's dtype, dequantized with one rounding from a
+    QuantizedKV. Slots outside the pool (-1) give zero rows."""
+    kv = _kv_struct(k_cache, v_cache)
+    slots = _i32(slots, "slots")
+    if slots.ndim != 1:
+        raise ValueError("slots must be [n]")
+    dev = k_cache.device
+    _on(dev, v_cache, slots)
+    n = slots.shape[0]
+    k, v = (torch.empty(n, kv.n_kv_heads, kv.head_dim, dtype=k_cache.dtype, device=dev)
+            for _ in range(2))
+    rc = _call(dev, lambda st: _lib.load().mlxq_kv_cache_read(kv, _p(slots), n, _p(k), _p(v), st))
+    _lib.check(rc, "kv_cache_read")
+    return k, v
+
+
+def _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, max_kv_len,
+                    tree_mask, scale, what):
+    """mlxq_paged_attention_rows: a cache of any width, one or several rows a sequence."""
+    kv = _kv_struct(k_cache, v_cache)
+    if q.ndim != 3 or q.dtype != k_cache.dtype or q.shape[2] != kv.head_dim:
+        raise ValueError("q must be [rows, n_heads, head_dim] of the cache's head_dim and dtype")
+    q = q.contiguous()
+    block_table, kv_lens = _i32(block_table, "block_table"), _i32(kv_lens, "kv_lens")
+    if block_table.ndim != 2 or kv_lens.shape != (block_table.shape[0],):
+        raise ValueError("block_table must be [B, max_blocks] and kv_lens [B]")
+    B = block_table.shape[0]
+    if cu_q is not None:
+        cu_q = _i32(cu_q, "cu_q")
+        if cu_q.shape != (B + 1,):
+            raise ValueError(f"cu_q must be [{B + 1}] (one offset per sequence, then the total)")
+    elif q.shape[0] != B:
+        raise ValueError(f"q must have one row per sequence ({B}), got {q.shape[0]}")
+    if tree_mask is not None:
+        if tree_mask.dtype != torch.int64 or tree_mask.shape != (q.shape[0],):
+            raise ValueError(f"tree_mask must be int64 [{q.shape[0]}]")
+        tree_mask = tree_mask.contiguous()
+    dev = q.device
+    _on(dev, cu_q, k_cache, v_cache, block_table, kv_lens, tree_mask)
+    out = torch.empty_like(q)
+    L = _lib.load()
+    rows, H, _ = q.shape
+    max_q_len, max_kv_len = int(max_q_len), int(max_kv_len)
+
+    def call(st):
+        need = L.mlxq_paged_attention_rows_workspace_size(kv, B, max_q_len, max_kv_len, H)
+        # per call, from the allocator: calls on other streams and in other captured graphs
+        # have their own
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        return L.mlxq_paged_attention_rows(kv, _p(q), _p(cu_q), rows, max_q_len, _p(block_table),
+                                           block_table.shape[1], _p(kv_lens), max_kv_len,
+                                           _p(tree_mask), _p(out), B, H, float(scale), _p(ws),
+                                           need, st)
+
+    _lib.check(_call(dev, call), what)
+    return out
+
+
+def paged_attention_tree(q: torch.Tensor, cu_q: torch.Tensor, max_q_len: int, k_cache, v_cache,
+                         block_table: torch.Tensor, kv_lens: torch.Tensor, max_kv_len: int,
+                         tree_mask: torch.Tensor, scale: float) -> torch.Tensor:
+    """Trees of drafted tokens: q [total, n_heads, head_dim], sequence b's n <= 64 tokens at
+    rows [cu_q[b], cu_q[b+1]), their keys and values appended as the last n of its
+    kv_lens[b] <= max_kv_len cached ones (slots in row order, whatever the tokens' depths
+    and positions). Every token sees the keys before those n, and of the n token j where
+    bit j of its word in tree_mask [total] (int64) is set: see tree_masks. A row that sees
+    nothing is zero, and so are rows behind cu_q[-1]. Caches of 16 bits or QuantizedKV."""
+    if tree_mask is None:
+        raise ValueError("paged_attention_tree needs a tree_mask")
+    return _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, max_kv_len,
+                           tree_mask, scale, "paged_attention_tree")
+
+
+def tree_masks(parents, device="cuda") -> torch.Tensor:
+    """Ancestor masks for paged_attention_tree from one list of parents per sequence (the
+    index of each token's parent, before it, in its own tree; -1 for a root): int64 [total],
+    each token's own bit and its ancestors'."""
+    masks = []
+    for tree in parents:
+        if len(tree) > 64:
+            raise ValueError("a tree has at most 64 tokens")
+        own = []
+        for i, p in enumerate(tree):
+            if not -1 <= p < i:
+                raise ValueError(f"token {i}'s parent must be an earlier token or -1, got {p}")
+            own.append((own[p] if p >= 0 else 0) | 1 << i)
+        masks += [m - (1 << 64) if m >> 63 else m for m in own]
+    return torch.tensor(masks, dtype=torch.int64, device=device)
+
+
 def _cache_geometry(k_cache, v_cache, q):
     if k_cache.shape != v_cache.shape or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise ValueError("k_cache and v_cache must share shape and q's dtype")
@@ -112,11 +336,15 @@ def _cache_geometry(k_cache, v_cache, q):
     return page, hkv, hd
 
 
-def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+def paged_attention_decode(q: torch.Tensor, k_cache, v_cache,
                            block_table: torch.Tensor, kv_lens: torch.Tensor, max_kv_len: int,
                            scale: float) -> torch.Tensor:
     """One query per sequence: q [B, n_heads, head_dim] at position kv_lens[b] - 1
-    attends all kv_lens[b] cached keys of sequence b (pages block_table[b])."""
+    attends all kv_lens[b] cached keys of sequence b (pages block_table[b]). The caches are
+    16-bit tensors or a pair of QuantizedKV."""
+    if isinstance(k_cache, QuantizedKV) or isinstance(v_cache, QuantizedKV):
+        return _rows_attention(q, None, 1, k_cache, v_cache, block_table, kv_lens, max_kv_len,
+                               None, scale, "paged_attention_decode")
     dt = _code(q, "q")
     page, hkv, hd = _cache_geometry(k_cache, v_cache, q)
     B, H, _ = q.shape
@@ -138,11 +366,17 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
 
 def paged_attention_prefill(q: torch.Tensor, cu_q: torch.Tensor, max_q_len: int,
-                            k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            k_cache, v_cache,
                             block_table: torch.Tensor, kv_lens: torch.Tensor,
                             scale: float) -> torch.Tensor:
     """New tokens of every sequence: q [total, n_heads, head_dim], sequence b's rows
-    [cu_q[b], cu_q[b+1]) at the last positions of its kv_lens[b] cached keys, causal."""
+    [cu_q[b], cu_q[b+1]) at the last positions of its kv_lens[b] cached keys, causal. The
+    caches are 16-bit tensors or a pair of QuantizedKV."""
+    if isinstance(k_cache, QuantizedKV) or isinstance(v_cache, QuantizedKV):
+        page = k_cache.shape[1]
+        return _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens,
+                               block_table.shape[-1] * page, None, scale,
+                               "paged_attention_prefill")
     dt = _code(q, "q")
     page, hkv, hd = _cache_geometry(k_cache, v_cache, q)
     _, H, _ = q.shape
@@ -213,16 +447,27 @@ class PagedBatch:
 class PagedKVCache:
     """Fixed-size page pools per layer, [num_pages, page_size, n_kv_heads, head_dim]
     for keys and for values (cache.py:651-700), and a free list of page ids handed
-    out to sequences in any order (the pages of a sequence need not be contiguous)."""
+    out to sequences in any order (the pages of a sequence need not be contiguous).
+    With bits 8 or 4 the pools are QuantizedKV, quantized in groups of group_size as
+    they are written."""
 
     def __init__(self, num_layers: int, n_kv_heads: int, head_dim: int, num_pages: int,
-                 page_size: int = 16, dtype=torch.bfloat16, device="cuda"):
+                 page_size: int = 16, dtype=torch.bfloat16, device="cuda", bits: int = 16,
+                 group_size: int = 64):
+        if bits not in (4, 8, 16):
+            raise ValueError("cache bits must be 4, 8 or 16")
         if page_size not in (8, 16, 32):
             raise ValueError("page_size must be 8, 16 or 32")
         self.page_size, self.n_kv_heads, self.head_dim = page_size, n_kv_heads, head_dim
         shape = (num_pages, page_size, n_kv_heads, head_dim)
-        self.keys = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
-        self.values = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        if bits == 16:
+            def pool():
+                return torch.zeros(shape, dtype=dtype, device=device)
+        else:
+            def pool():
+                return QuantizedKV.zeros(*shape, group_size, bits, dtype, device)
+        self.keys = [pool() for _ in range(num_layers)]
+        self.values = [pool() for _ in range(num_layers)]
         self._free = list(range(num_pages))
         self._lock = threading.Lock()
 

@@ -1,0 +1,567 @@
+// Attention of query rows over a paged KV cache in 16, 8 or 4 bits (sm_100a): decode steps,
+// prompt chunks and trees of drafted tokens.
+//
+// Reference (huydt84/mlx-server-runtime, python/mlx_worker/native_mlx/): append_and_attend
+// (attention.py:215-298) over pages, with a causal or, for drafted trees, an ancestor mask.
+//
+//   s = scale * q . k over the visible keys, p = exp(s - m), out = sum p v / sum p
+//
+// Rows: sequence b has R = n * G query rows per kv head (its n new tokens times the G query
+// heads that share the head). They are taken in chunks of ROWS; the chunk's keys in tiles
+// of 64. The tiles of all (sequence, kv head, chunk) items form one sequence of units that
+// the CTAs share out evenly, whatever the lengths: a CTA's share is a contiguous run that
+// may end one item and begin another. A part of an item goes to a workspace slot of its
+// CTA, and attn_combine_kernel joins the parts in order of keys.
+//
+// Keys are the M rows of the m16n8k16 products and query rows the N columns, so eight rows
+// (a decode step's heads) fill a tile without padding:
+//   S^T = K Q^T    A = 16 keys x 16 dims, straight from global memory: a lane's dims are
+//                  contiguous in its key's row, and q is permuted to match once
+//   O^T = V^T P^T  A = 16 dims x 16 keys, pairs of keys joined by byte permutes; P^T is S^T
+//                  rounded to T and transposed in registers (movmatrix)
+// so packed codes go from their load through registers into the product; shared memory
+// holds only the four warps' results at the end of an item.
+#include "common.cuh"
+#include "kv_dequant.cuh"
+#include "overlap.cuh"
+#include "paged_ops.h"
+#include "sm100.cuh"
+
+namespace mlxq {
+
+namespace ra {
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int KT = 16 * WARPS;  // keys per tile
+
+struct Params {
+    RowsArgs a;
+    KvCache c;
+    float scale_log2;
+    float* part_o;    // [2 P][ROWS][HD]
+    float2* part_ml;  // [2 P][ROWS] running max (base 2) and sum
+    int parts;        // P: CTAs the units are shared out to
+};
+
+// One sequence's place in the batch, with everything a bad length or offset could do bounded.
+struct Seq {
+    int row0, n, L, chunks, tiles;
+};
+__device__ __forceinline__ Seq seq_of(const RowsArgs& a, int b, int G, int rows) {
+    Seq s;
+    int lo = b, hi = b + 1;
+    if (a.cu_q) {
+        lo = a.cu_q[b];
+        hi = a.cu_q[b + 1];
+    }
+    s.row0 = max(0, min(lo, a.total));
+    s.n = max(0, min(min(hi, a.total) - s.row0, a.max_q));
+    s.L = max(0, min(a.kv_lens[b], a.max_kv));
+    s.chunks = (s.n * G + rows - 1) / rows;
+    s.tiles = max(1, (s.L + KT - 1) / KT);  // a sequence without keys still writes its zeros
+    return s;
+}
+
+// Prefix sums of the batch's units, each thread over a run of sequences.
+struct Units {
+    long long total;
+    int per;  // sequences per thread
+};
+__device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, int rows,
+                                            long long* pref /* [THREADS + 1] */) {
+    __shared__ long long wsum[WARPS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Units u;
+    u.per = (a.batch + THREADS - 1) / THREADS;
+    long long sum = 0;
+    for (int b = tid * u.per; b < min(a.batch, (tid + 1) * u.per); ++b) {
+        const Seq s = seq_of(a, b, G, rows);
+        sum += static_cast<long long>(s.chunks) * s.tiles * Hkv;
+    }
+    long long inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) inc += wsum[w];
+    pref[tid + 1] = inc;
+    if (tid == 0) pref[0] = 0;
+    __syncthreads();
+    u.total = pref[THREADS];
+    return u;
+}
+// Sequence that holds unit x, and the unit its first item starts at.
+__device__ __forceinline__ int find_seq(const RowsArgs& a, int Hkv, int G, int rows,
+                                        const long long* pref, int per, long long x,
+                                        long long& start) {
+    int lo = 0, hi = THREADS - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pref[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    start = pref[lo];
+    int b = lo * per;
+    for (; b + 1 < a.batch; ++b) {
+        const Seq s = seq_of(a, b, G, rows);
+        const long long n = static_cast<long long>(s.chunks) * s.tiles * Hkv;
+        if (x < start + n) break;
+        start += n;
+    }
+    return b;
+}
+// CTA that owns unit x of `total` shared out to P.
+__device__ __forceinline__ int owner(long long x, long long total, int P) {
+    return static_cast<int>(((x + 1) * P - 1) / total);
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+    return r;
+}
+
+template <int N>
+__device__ __forceinline__ void ldw(const uint32_t* p, uint32_t (&r)[N]) {
+    if constexpr (N == 1) {
+        r[0] = *p;
+    } else if constexpr (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        r[0] = v.x;
+        r[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            r[4 * i] = v.x;
+            r[4 * i + 1] = v.y;
+            r[4 * i + 2] = v.z;
+            r[4 * i + 3] = v.w;
+        }
+    }
+}
+}  // namespace ra
+
+template <typename T, int HD, int BITS, int NT>
+__global__ void __launch_bounds__(ra::THREADS)
+    attn_rows_kernel(const __grid_constant__ ra::Params p) {
+    using namespace ra;
+    constexpr int ROWS = 8 * NT;
+    constexpr int KW = HD / 4 * BITS / 32;  // words of a key row per lane (a quarter)
+    constexpr int VW = HD / 8 * BITS / 32;  // words of a value row per lane (an eighth)
+    constexpr int RW = HD * BITS / 32;      // words of a row
+    constexpr int MT = HD / 16;
+    __shared__ long long pref[THREADS + 1];
+    __shared__ float wo[WARPS][ROWS][HD + 4];
+    __shared__ float wm[WARPS][ROWS], wl[WARPS][ROWS];
+    pdl_launch_dependents();
+    pdl_wait();
+    const RowsArgs& a = p.a;
+    const KvCache& c = p.c;
+    const int Hkv = c.Hkv, G = a.Hq / Hkv;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, c4 = lane & 3;
+    const T* q = static_cast<const T*>(a.q);
+    T* out = static_cast<T*>(a.out);
+
+    if (a.cu_q) {  // rows behind the last sequence are zero
+        const long long row = static_cast<long long>(a.Hq) * HD / 8;
+        const int end = max(0, min(a.cu_q[a.batch], a.total));
+        uint4* o = reinterpret_cast<uint4*>(out);
+        for (long long i = end * row + blockIdx.x * THREADS + tid; i < a.total * row;
+             i += static_cast<long long>(gridDim.x) * THREADS)
+            o[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    const Units un = scan_units(a, Hkv, G, ROWS, pref);
+    const int P = static_cast<int>(min(static_cast<long long>(p.parts), un.total));
+    if (static_cast<int>(blockIdx.x) >= P) return;
+    long long u = un.total * blockIdx.x / P;  // (P <= total: no share is empty)
+    const long long u_lo = u, u_hi = un.total * (blockIdx.x + 1) / P;
+    long long start;
+    int b = find_seq(a, Hkv, G, ROWS, pref, un.per, u, start);
+
+    const uint32_t* kd = static_cast<const uint32_t*>(c.k);
+    const uint32_t* vd = static_cast<const uint32_t*>(c.v);
+    const uint16_t *ksd = static_cast<const uint16_t*>(c.ks), *kbd = static_cast<const uint16_t*>(c.kb);
+    const uint16_t *vsd = static_cast<const uint16_t*>(c.vs), *vbd = static_cast<const uint16_t*>(c.vb);
+    const int ng = BITS == 16 ? 1 : HD / c.gs;
+    const int kg = BITS == 16 ? 0 : c4 * (HD / 4) / c.gs;  // this lane's group of a key row
+    const int vg = BITS == 16 ? 0 : r8 * (HD / 8) / c.gs;  // and of a value row
+
+    while (u < u_hi) {
+        const Seq s = seq_of(a, b, G, ROWS);
+        const long long seq_units = static_cast<long long>(s.chunks) * s.tiles * Hkv;
+        if (u >= start + seq_units) {
+            start += seq_units;
+            ++b;
+            continue;
+        }
+        // the item: kv head fastest outside the tiles, so that neighbouring shares read
+        // neighbouring parts of the same pages
+        const int item = static_cast<int>((u - start) / s.tiles);
+        const int t0 = static_cast<int>((u - start) % s.tiles);
+        const int t1 = static_cast<int>(min(static_cast<long long>(s.tiles), t0 + (u_hi - u)));
+        const int g = item % Hkv, chunk = item / Hkv;
+        const int row_lo = chunk * ROWS, R = s.n * G;
+        const int base = s.L - s.n;  // keys before it are seen by every row
+        const int32_t* bt = a.table + static_cast<size_t>(b) * a.max_blocks;
+
+        // Queries: lane (row r8 of the n-tile, quarter c4) holds its quarter's dims in the
+        // order the key words unpack to.
+        uint32_t bq[NT][MT][2];
+        int qpos[NT][2];              // column 2 c4 + e: its index among the new tokens
+        unsigned long long vis[NT][2];  // and its ancestors
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int rr = row_lo + 8 * nt + r8;
+            uint32_t w[HD / 8];
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) w[i] = 0u;
+            if (rr < R)
+                ldw(reinterpret_cast<const uint32_t*>(
+                        q + (static_cast<size_t>(s.row0 + rr / G) * a.Hq + g * G + rr % G) * HD +
+                        c4 * (HD / 4)),
+                    w);
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) {
+                const int da = pair_dim<BITS>(i, 0), db = pair_dim<BITS>(i, 1);
+                bq[nt][i / 2][i % 2] =
+                    prmt(w[da / 2], w[db / 2], (da % 2 ? 0x32u : 0x10u) | (db % 2 ? 0x7600u : 0x5400u));
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int rc = row_lo + 8 * nt + 2 * c4 + e;
+                qpos[nt][e] = rc < R ? rc / G : -1;
+                vis[nt][e] = ~0ull;
+                if (a.mask) vis[nt][e] = rc < R ? static_cast<unsigned long long>(a.mask[s.row0 + rc / G]) : 0ull;
+            }
+        }
+        // keys the chunk can see: with a causal mask, those up to its last row
+        const int last = min(R, row_lo + ROWS) - 1;
+        const int kend = max(0, a.mask ? s.L : min(s.L, base + last / G + 1));
+        const int full = min(max(base, 0), kend);  // keys every row sees
+
+        float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
+
+        // One 16-key tile per warp and step; the next tile's words are loaded while this
+        // one is multiplied.
+        uint32_t kw[2][KW], vw[4][VW], ksb[2], vsb[2][2];  // (scale, bias) / pairs of keys
+        bool okk[2];
+        auto load = [&](int tile) {
+            const int k0 = tile * KT + warp * 16;
+            const uint32_t *kr[2], *vr[2];
+            size_t row[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // eight keys share a page
+                const int key = k0 + 8 * h;
+                int pid = -1;
+                if (key < kend) pid = bt[key / c.page];
+                okk[h] = pid >= 0 && pid < c.pages;
+                row[h] = okk[h] ? (static_cast<size_t>(pid) * c.page + key % c.page) * Hkv + g
+                                : static_cast<size_t>(g);
+                kr[h] = kd + (row[h] + (okk[h] ? static_cast<size_t>(r8) * Hkv : 0)) * RW + c4 * KW;
+                vr[h] = vd + (row[h] + (okk[h] ? static_cast<size_t>(2 * c4) * Hkv : 0)) * RW + r8 * VW;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                ldw(kr[h], kw[h]);
+                ldw(vr[h], vw[2 * h]);
+                ldw(vr[h] + (okk[h] ? static_cast<size_t>(Hkv) * RW : 0), vw[2 * h + 1]);
+            }
+            if constexpr (BITS != 16) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const size_t ki = (row[h] + (okk[h] ? static_cast<size_t>(r8) * Hkv : 0)) * ng + kg;
+                    ksb[h] = ksd[ki] | static_cast<uint32_t>(kbd[ki]) << 16;
+                    const size_t step = okk[h] ? static_cast<size_t>(Hkv) * ng : 0;
+                    const size_t vi = row[h] * ng + vg + 2 * c4 * step;
+                    vsb[h][0] = vsd[vi] | static_cast<uint32_t>(vsd[vi + step]) << 16;
+                    vsb[h][1] = vbd[vi] | static_cast<uint32_t>(vbd[vi + step]) << 16;
+                }
+            }
+        };
+        const int te = min(t1, (kend + KT - 1) / KT);
+        if (t0 < te) load(t0);
+        for (int tile = t0; tile < te; ++tile) {
+            const int k0 = tile * KT + warp * 16;
+            // values of keys that are not there multiply zeros: make them zeros
+            const bool clean = k0 + 16 <= kend && okk[0] && okk[1];
+            if (!clean) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = k0 + 8 * h + 2 * c4;
+                    const uint32_t keep = (okk[h] && k < kend ? 0xffffu : 0u) |
+                                          (okk[h] && k + 1 < kend ? 0xffff0000u : 0u);
+                    if constexpr (BITS == 16) {
+#pragma unroll
+                        for (int i = 0; i < VW; ++i) {
+                            if (!(keep & 0xffffu)) vw[2 * h][i] = 0u;
+                            if (!(keep >> 16)) vw[2 * h + 1][i] = 0u;
+                        }
+                    } else {
+                        vsb[h][0] &= keep;
+                        vsb[h][1] &= keep;
+                    }
+                }
+            }
+            float sc[NT][4];
+            uint32_t va[MT][4];
+            {
+                const uint32_t s0 = pk_splat(ksb[0]), b0 = prmt(ksb[0], 0u, 0x3232u);
+                const uint32_t s1 = pk_splat(ksb[1]), b1 = prmt(ksb[1], 0u, 0x3232u);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) {
+                    const uint32_t a0 = row_pair<T, BITS>(kw[0], 2 * j, s0, b0);
+                    const uint32_t a1 = row_pair<T, BITS>(kw[1], 2 * j, s1, b1);
+                    const uint32_t a2 = row_pair<T, BITS>(kw[0], 2 * j + 1, s0, b0);
+                    const uint32_t a3 = row_pair<T, BITS>(kw[1], 2 * j + 1, s1, b1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        if (j == 0) mma16816z<T>(sc[nt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
+                        else mma16816<T>(sc[nt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    va[i][0] = cross_pair<T, BITS>(vw[0], vw[1], i, vsb[0][0], vsb[0][1]);
+                    va[i][1] = cross_pair<T, BITS>(vw[0], vw[1], MT + i, vsb[0][0], vsb[0][1]);
+                    va[i][2] = cross_pair<T, BITS>(vw[2], vw[3], i, vsb[1][0], vsb[1][1]);
+                    va[i][3] = cross_pair<T, BITS>(vw[2], vw[3], MT + i, vsb[1][0], vsb[1][1]);
+                }
+            }
+            const bool ok0 = okk[0], ok1 = okk[1];
+            if (tile + 1 < te) load(tile + 1);
+            const bool plain = clean && k0 + 16 <= full;
+            float grow = -INFINITY;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = sc[nt][e] * p.scale_log2;
+                    if (!plain) {
+                        const int key = k0 + r8 + 8 * (e >> 1), j = key - base;
+                        const bool see = key < kend && ((e >> 1) ? ok1 : ok0) &&
+                                         (j < 0 || (a.mask ? j < 64 && (vis[nt][e & 1] >> (j & 63) & 1)
+                                                           : j <= qpos[nt][e & 1]));
+                        x = see ? x : -INFINITY;
+                    }
+                    sc[nt][e] = x;
+                    grow = fmaxf(grow, x - m[nt][e & 1]);
+                }
+            // The reference of the exponentials follows the running maximum only when a
+            // score passes it by 2^8: the probabilities then reach 256, the sums lose nothing.
+            if (__any_sync(0xffffffffu, grow > 8.f)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(sc[nt][e], sc[nt][e + 2]);
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                        mx = fmaxf(mx, m[nt][e]);
+                        const float f = mx == -INFINITY ? 1.f : exp2f(m[nt][e] - mx);
+                        m[nt][e] = mx;
+                        l[nt][e] *= f;
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) {
+                            o[nt][i][e] *= f;
+                            o[nt][i][e + 2] *= f;
+                        }
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float pr[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mr = m[nt][e & 1];
+                    pr[e] = exp2f(sc[nt][e] - (mr == -INFINITY ? 0.f : mr));
+                    l[nt][e & 1] += pr[e];
+                }
+                const uint32_t b0 = transpose8x8(pk_round<T>(pr[0], pr[1]));
+                const uint32_t b1 = transpose8x8(pk_round<T>(pr[2], pr[3]));
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    mma16816<T>(o[nt][i], va[i][0], va[i][1], va[i][2], va[i][3], b0, b1);
+            }
+        }
+
+        // Join the warps: (max, sum, O) of every row through shared memory.
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[nt][e];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int col = 8 * nt + 2 * c4 + e;
+                if (r8 == 0) {
+                    wm[warp][col] = m[nt][e];
+                    wl[warp][col] = sum;
+                }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    wo[warp][col][r8 * (HD / 8) + i] = o[nt][i][e];
+                    wo[warp][col][r8 * (HD / 8) + MT + i] = o[nt][i][e + 2];
+                }
+            }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == s.tiles;
+        const size_t slot = (2 * static_cast<size_t>(blockIdx.x) + (u == u_lo ? 0 : 1)) * ROWS;
+        for (int i = tid; i < ROWS * HD / 2; i += THREADS) {
+            const int row = i / (HD / 2), d = 2 * (i % (HD / 2)), rr = row_lo + row;
+            if (rr >= R) continue;
+            float M = -INFINITY, den = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) M = fmaxf(M, wm[w][row]);
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = wm[w][row] == -INFINITY ? 0.f : exp2f(wm[w][row] - M);
+                den = fmaf(f, wl[w][row], den);
+                x = fmaf(f, wo[w][row][d], x);
+                y = fmaf(f, wo[w][row][d + 1], y);
+            }
+            if (whole) {
+                const float inv = M == -INFINITY ? 0.f : 1.0f / den;
+                T* dst = out + (static_cast<size_t>(s.row0 + rr / G) * a.Hq + g * G + rr % G) * HD + d;
+                *reinterpret_cast<uint32_t*>(dst) = pk_round<T>(x * inv, y * inv);
+            } else {
+                *reinterpret_cast<float2*>(p.part_o + (slot + row) * HD + d) = make_float2(x, y);
+                if (d == 0) p.part_ml[slot + row] = make_float2(M, den);
+            }
+        }
+        __syncthreads();  // the shared results are read before the next item writes its own
+        u += t1 - t0;
+    }
+}
+
+// Joins the parts of the items that were shared among CTAs: block (item of the whole
+// batch, row of its chunk), thread = dimension. Parts are taken in order of keys.
+template <typename T, int HD, int ROWS>
+__global__ void __launch_bounds__(ra::THREADS)
+    attn_combine_kernel(const __grid_constant__ ra::Params p) {
+    using namespace ra;
+    __shared__ long long pref[THREADS + 1];
+    pdl_launch_dependents();
+    pdl_wait();
+    const RowsArgs& a = p.a;
+    const int Hkv = p.c.Hkv, G = a.Hq / Hkv;
+    const Units un = scan_units(a, Hkv, G, ROWS, pref);
+    const int P = static_cast<int>(min(static_cast<long long>(p.parts), un.total));
+    // an item that was cut holds some CTA's first or last unit: block (boundary i, row)
+    // takes the item that unit u_lo(i) lies inside of, if boundary i is its first
+    const int i = blockIdx.x + 1;
+    if (i >= P) return;
+    const long long x = un.total * i / P;
+    long long start;
+    const int b = find_seq(a, Hkv, G, ROWS, pref, un.per, x, start);
+    const Seq s = seq_of(a, b, G, ROWS);
+    const int item = static_cast<int>((x - start) / s.tiles);
+    const long long u0 = start + static_cast<long long>(item) * s.tiles;
+    if (x == u0) return;                     // the boundary is the item's own beginning
+    if (un.total * (i - 1) / P > u0) return; // an earlier boundary cuts the same item
+    const int g = item % Hkv, rr = item / Hkv * ROWS + static_cast<int>(blockIdx.y);
+    if (rr >= s.n * G) return;
+    const int first = owner(u0, un.total, P), lastc = owner(u0 + s.tiles - 1, un.total, P);
+    const int d = threadIdx.x;
+    float M = -INFINITY, den = 0.f, acc = 0.f;
+#pragma unroll 4
+    for (int k = first; k <= lastc; ++k) {
+        const size_t slot = (2 * static_cast<size_t>(k) + (un.total * k / P >= u0 ? 0 : 1)) * ROWS +
+                            blockIdx.y;
+        const float2 ml = p.part_ml[slot];
+        const float v = d < HD ? p.part_o[slot * HD + d] : 0.f;
+        const float Mn = fmaxf(M, ml.x);
+        const float co = M == -INFINITY ? 0.f : exp2f(M - Mn);
+        const float cn = ml.x == -INFINITY ? 0.f : exp2f(ml.x - Mn);
+        den = fmaf(cn, ml.y, den * co);
+        acc = fmaf(cn, v, acc * co);
+        M = Mn;
+    }
+    if (d < HD)
+        static_cast<T*>(a.out)[(static_cast<size_t>(s.row0 + rr / G) * a.Hq + g * G + rr % G) * HD + d] =
+            Elem<T>::from_f(M == -INFINITY ? 0.f : acc / den);
+}
+
+namespace {
+
+// Query rows per chunk: a decode step's heads fit one n-tile of eight.
+int n_tiles(const KvCache& c, const RowsArgs& a) { return a.max_q * (a.Hq / c.Hkv) <= 8 ? 1 : 2; }
+
+// CTAs the units are shared out to: what the GPU holds at once (four CTAs of four warps
+// per SM with one n-tile, two with two), at most one per unit.
+int parts_of(const KvCache& c, const RowsArgs& a) {
+    const int nt = n_tiles(c, a), rows = 8 * nt;
+    const long long chunks = (static_cast<long long>(a.max_q) * (a.Hq / c.Hkv) + rows - 1) / rows;
+    const long long tiles = (a.max_kv + ra::KT - 1) / ra::KT;
+    long long units = chunks * (tiles > 0 ? tiles : 1) * c.Hkv;
+    const long long most = 148LL * (nt == 1 ? 4 : 2);
+    if (units > most) return static_cast<int>(most);
+    units *= a.batch;
+    return static_cast<int>(units < most ? (units > 0 ? units : 1) : most);
+}
+
+template <typename T, int HD, int BITS>
+const void* rows_fn(int nt) {
+    return nt == 1 ? reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 1>)
+                   : reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 2>);
+}
+template <typename T, int HD>
+const void* rows_fn(int bits, int nt) {
+    return bits == 16 ? rows_fn<T, HD, 16>(nt) : bits == 8 ? rows_fn<T, HD, 8>(nt) : rows_fn<T, HD, 4>(nt);
+}
+template <typename T>
+const void* combine_fn(int hd, int nt) {
+    if (hd == 128)
+        return nt == 1 ? reinterpret_cast<const void*>(&attn_combine_kernel<T, 128, 8>)
+                       : reinterpret_cast<const void*>(&attn_combine_kernel<T, 128, 16>);
+    return nt == 1 ? reinterpret_cast<const void*>(&attn_combine_kernel<T, 64, 8>)
+                   : reinterpret_cast<const void*>(&attn_combine_kernel<T, 64, 16>);
+}
+
+}  // namespace
+
+size_t attn_rows_workspace(const KvCache& c, const RowsArgs& a) {
+    const size_t slots = 2 * static_cast<size_t>(parts_of(c, a)) * 8 * n_tiles(c, a);
+    return slots * (c.hd * sizeof(float) + sizeof(float2));
+}
+
+cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspace, bool overlap,
+                             cudaStream_t st) {
+    const int nt = n_tiles(c, a), P = parts_of(c, a);
+    ra::Params p;
+    p.a = a;
+    p.c = c;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.parts = P;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + 2 * static_cast<size_t>(P) * 8 * nt * c.hd);
+    void* args[] = {&p};
+    const bool bf = c.dtype == kBF16;
+    const void* f = bf ? (c.hd == 128 ? rows_fn<__nv_bfloat16, 128>(c.bits, nt)
+                                      : rows_fn<__nv_bfloat16, 64>(c.bits, nt))
+                       : (c.hd == 128 ? rows_fn<__half, 128>(c.bits, nt)
+                                      : rows_fn<__half, 64>(c.bits, nt));
+    static PerDevice cfg[24];
+    const int which = (((bf ? 0 : 1) * 2 + (c.hd == 128 ? 0 : 1)) * 3 +
+                       (c.bits == 16 ? 0 : c.bits == 8 ? 1 : 2)) * 2 + nt - 1;
+    cudaError_t e = launch_ex(f, cfg[which], dim3(P), dim3(ra::THREADS), 0, st, overlap, args);
+    if (e != cudaSuccess || P == 1) return e;
+    const void* fc = bf ? combine_fn<__nv_bfloat16>(c.hd, nt) : combine_fn<__half>(c.hd, nt);
+    static PerDevice cfgc[8];
+    // (its launch may begin while the parts are computed; it waits for them all)
+    return launch_ex(fc, cfgc[((bf ? 0 : 1) * 2 + (c.hd == 128 ? 0 : 1)) * 2 + nt - 1],
+                     dim3(P - 1, 8 * nt), dim3(ra::THREADS), 0, st, true, args);
+}
+
+}  // namespace mlxq

@@ -9,6 +9,7 @@
 // in the reference: mx.quantize at lfm2.py:112-117, nn.quantize at qwen2.py:318-324).
 #include "common.cuh"
 #include "launch.h"
+#include "quant_rule.cuh"
 
 namespace mlxq {
 
@@ -65,28 +66,6 @@ __device__ __forceinline__ void store_words(void* p, const uint32_t (&r)[N]) {
     }
 }
 
-// The code of one element, clamp(rint(RN(d / s)), 0, n_bins) with RN the IEEE
-// quotient, from r = RN(1 / s): q = RN(d * r) is within (2^-23 + 2^-48) |d / s| of
-// d / s, and RN(d / s) within 2^-24 |d / s|, so for |q| <= 1024 the two differ by
-// less than 2e-4. When q is more than 1e-3 from every half-integer, both round to
-// the same integer; otherwise (or when q is outside [-1024, 1024], not a number, or
-// r is not a normal float: `fast` false) the IEEE quotient is taken.
-// Rounding to an integer adds and subtracts 1.5 * 2^23 (a float in [2^23, 2^24) has
-// unit spacing, and the add rounds to nearest even like rintf for |q| < 2^22), and the
-// clamped integer is read from the low mantissa bits of the same sum: no conversion
-// instructions on the common path.
-constexpr float kRoundMagic = 12582912.0f;  // 1.5 * 2^23
-constexpr uint32_t kRoundMagicBits = 0x4B400000u;
-
-__device__ __forceinline__ uint32_t quant_code(float d, float s, float r, float n_bins, bool fast) {
-    const float q = __fmul_rn(d, r);
-    float k = __fsub_rn(__fadd_rn(q, kRoundMagic), kRoundMagic);
-    if (!fast || !(fabsf(q) <= 1024.0f) || fabsf(__fsub_rn(q, k)) > 0.499f)
-        k = rintf(__fdiv_rn(d, s));
-    k = fminf(fmaxf(k, 0.0f), n_bins);
-    return __float_as_uint(__fadd_rn(k, kRoundMagic)) - kRoundMagicBits;
-}
-
 // One thread quantizes WPT consecutive packed words (WPT * 32/bits elements, all in
 // one group); the group_size / (WPT * 32/bits) threads of a group sit in adjacent
 // lanes, so group min/max is a shuffle reduction over them, and the group's scale
@@ -128,17 +107,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ w,
     }
     if (!live) return;
 
-    const bool mask = fabsf(lmin) > fabsf(lmax);
-    float scale = __fdiv_rn(__fsub_rn(lmax, lmin), n_bins);
-    scale = fmaxf(scale, 1e-7f);
-    scale = mask ? scale : -scale;
-    const float edge = mask ? lmin : lmax;
-    const float q0 = rintf(__fdiv_rn(edge, scale));
-    float bias = 0.0f;
-    if (q0 != 0.0f) {
-        scale = __fdiv_rn(edge, q0);
-        bias = edge;
-    }
+    float scale, bias;
+    quant_group(lmin, lmax, n_bins, scale, bias);
     const float r = __frcp_rn(scale);
     const float ar = fabsf(r);
     const bool fast = ar >= 0x1p-126f && ar <= 0x1p126f;

@@ -44,6 +44,7 @@ class Qwen2Config:
     tie_word_embeddings: bool = False
     group_size: int = 64
     bits: int = 4
+    qk_norm: bool = False   # RMSNorm of each query and key head before the rotation
 
     @property
     def head_dim(self) -> int:
@@ -61,7 +62,8 @@ class Qwen2Attention(nn.Module):
     """q/k/v projections (with bias) stacked into one quantized launch, RoPE and the
     paged KV append in one kernel, paged attention, then o_proj (qwen2.py:46-118)."""
 
-    def __init__(self, cfg: Qwen2Config, *, device, dtype, generator, bias_std=0.0):
+    def __init__(self, cfg: Qwen2Config, *, device, dtype, generator, norm_jitter=0.0,
+                 bias_std=0.0):
         D, hd = cfg.hidden_size, cfg.head_dim
         self.n_heads, self.n_kv_heads, self.head_dim = (cfg.num_attention_heads,
                                                         cfg.num_key_value_heads, hd)
@@ -78,13 +80,19 @@ class Qwen2Attention(nn.Module):
                                                  generator=generator)).to(dtype)
         self.qkv_proj = nn.FusedQuantizedLinear([q, k, v])
         self.o_proj = nn.QuantizedLinear(self.n_heads * hd, D, bias=False, **kw)
+        self.q_norm = self.k_norm = None
+        self.eps = cfg.rms_norm_eps
+        if cfg.qk_norm:
+            self.q_norm = _norm_weight(hd, device, dtype, generator, norm_jitter)
+            self.k_norm = _norm_weight(hd, device, dtype, generator, norm_jitter)
 
     def __call__(self, x, batch: PagedBatch, k_cache, v_cache):
         f = self.qkv_proj
         qkv = core.quantized_matmul(x, f.weight, f.scales, f.biases, True, f.group_size, f.bits,
                                     f.mode, bias=f.bias)
         q = rope_kv_append(qkv, batch.positions, batch.slots, k_cache, v_cache, self.n_heads,
-                           self.n_kv_heads, self.head_dim, self.rope_base)
+                           self.n_kv_heads, self.head_dim, self.rope_base, self.q_norm,
+                           self.k_norm, self.eps)
         if batch.cu_q is None:
             a = paged_attention_decode(q, k_cache, v_cache, batch.block_table, batch.kv_lens,
                                        batch.max_kv_len, self.scale)
@@ -119,7 +127,7 @@ class Qwen2TransformerBlock(nn.Module):
     def __init__(self, cfg: Qwen2Config, *, device, dtype, generator, norm_jitter=0.0,
                  bias_std=0.0):
         self.self_attn = Qwen2Attention(cfg, device=device, dtype=dtype, generator=generator,
-                                        bias_std=bias_std)
+                                        norm_jitter=norm_jitter, bias_std=bias_std)
         self.mlp = Qwen2Mlp(cfg, device=device, dtype=dtype, generator=generator)
         self.input_layernorm = _norm_weight(cfg.hidden_size, device, dtype, generator,
                                             norm_jitter)
