@@ -12,6 +12,7 @@
 
 #include "../../include/mlxq_b200.h"
 #include "launch.h"
+#include "paged_ops.h"
 
 namespace {
 
@@ -148,11 +149,12 @@ int mlxq_get_launch_overlap(void) { return g_overlap.load(); }
 int mlxq_device_error(int* code) {
     if (!code) return fail(MLXQ_ERR_NULL, "device_error: NULL pointer");
     *code = 0;
-    int a = 0, b = 0;
+    int a = 0, b = 0, r = 0;
     cudaError_t e = mlxq::qgemm_read_error(&a);
     if (e == cudaSuccess) e = mlxq::qmv_tma_read_error(&b);
+    if (e == cudaSuccess) e = mlxq::rows_tc_read_error(&r);
     if (e != cudaSuccess) return cuda_fail(e, "device_error");
-    *code = a ? a : b;
+    *code = a ? a : b ? b : r;
     return MLXQ_OK;
 }
 

@@ -25,6 +25,7 @@
 #include "kv_dequant.cuh"
 #include "overlap.cuh"
 #include "paged_ops.h"
+#include "rows_units.cuh"
 #include "sm100.cuh"
 
 namespace mlxq {
@@ -32,90 +33,6 @@ namespace mlxq {
 namespace ra {
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int KT = 16 * WARPS;  // keys per tile
-
-struct Params {
-    RowsArgs a;
-    KvCache c;
-    float scale_log2;
-    float* part_o;    // [2 P][ROWS][HD]
-    float2* part_ml;  // [2 P][ROWS] running max (base 2) and sum
-    int parts;        // P: CTAs the units are shared out to
-};
-
-// One sequence's place in the batch, with everything a bad length or offset could do bounded.
-struct Seq {
-    int row0, n, L, chunks, tiles;
-};
-__device__ __forceinline__ Seq seq_of(const RowsArgs& a, int b, int G, int rows) {
-    Seq s;
-    int lo = b, hi = b + 1;
-    if (a.cu_q) {
-        lo = a.cu_q[b];
-        hi = a.cu_q[b + 1];
-    }
-    s.row0 = max(0, min(lo, a.total));
-    s.n = max(0, min(min(hi, a.total) - s.row0, a.max_q));
-    s.L = max(0, min(a.kv_lens[b], a.max_kv));
-    s.chunks = (s.n * G + rows - 1) / rows;
-    s.tiles = max(1, (s.L + KT - 1) / KT);  // a sequence without keys still writes its zeros
-    return s;
-}
-
-// Prefix sums of the batch's units, each thread over a run of sequences.
-struct Units {
-    long long total;
-    int per;  // sequences per thread
-};
-__device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, int rows,
-                                            long long* pref /* [THREADS + 1] */) {
-    __shared__ long long wsum[WARPS];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    Units u;
-    u.per = (a.batch + THREADS - 1) / THREADS;
-    long long sum = 0;
-    for (int b = tid * u.per; b < min(a.batch, (tid + 1) * u.per); ++b) {
-        const Seq s = seq_of(a, b, G, rows);
-        sum += static_cast<long long>(s.chunks) * s.tiles * Hkv;
-    }
-    long long inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-    }
-    if (lane == 31) wsum[warp] = inc;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) inc += wsum[w];
-    pref[tid + 1] = inc;
-    if (tid == 0) pref[0] = 0;
-    __syncthreads();
-    u.total = pref[THREADS];
-    return u;
-}
-// Sequence that holds unit x, and the unit its first item starts at.
-__device__ __forceinline__ int find_seq(const RowsArgs& a, int Hkv, int G, int rows,
-                                        const long long* pref, int per, long long x,
-                                        long long& start) {
-    int lo = 0, hi = THREADS - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pref[mid] <= x) lo = mid;
-        else hi = mid - 1;
-    }
-    start = pref[lo];
-    int b = lo * per;
-    for (; b + 1 < a.batch; ++b) {
-        const Seq s = seq_of(a, b, G, rows);
-        const long long n = static_cast<long long>(s.chunks) * s.tiles * Hkv;
-        if (x < start + n) break;
-        start += n;
-    }
-    return b;
-}
-// CTA that owns unit x of `total` shared out to P.
-__device__ __forceinline__ int owner(long long x, long long total, int P) {
-    return static_cast<int>(((x + 1) * P - 1) / total);
-}
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -165,21 +82,11 @@ __global__ void __launch_bounds__(ra::THREADS)
     const T* q = static_cast<const T*>(a.q);
     T* out = static_cast<T*>(a.out);
 
-    if (a.cu_q) {  // rows behind the last sequence are zero
-        const long long row = static_cast<long long>(a.Hq) * HD / 8;
-        const int end = max(0, min(a.cu_q[a.batch], a.total));
-        uint4* o = reinterpret_cast<uint4*>(out);
-        for (long long i = end * row + blockIdx.x * THREADS + tid; i < a.total * row;
-             i += static_cast<long long>(gridDim.x) * THREADS)
-            o[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    const Units un = scan_units(a, Hkv, G, ROWS, pref);
-    const int P = static_cast<int>(min(static_cast<long long>(p.parts), un.total));
-    if (static_cast<int>(blockIdx.x) >= P) return;
-    long long u = un.total * blockIdx.x / P;  // (P <= total: no share is empty)
-    const long long u_lo = u, u_hi = un.total * (blockIdx.x + 1) / P;
-    long long start;
-    int b = find_seq(a, Hkv, G, ROWS, pref, un.per, u, start);
+    zero_tail(a, HD, THREADS);
+    const Units un = scan_units<KT>(a, Hkv, G, ROWS, pref);
+    Walk<KT, ROWS> w;
+    w.begin(a, Hkv, un, p.parts, pref);
+    Cut mine = {};
 
     const uint32_t* kd = static_cast<const uint32_t*>(c.k);
     const uint32_t* vd = static_cast<const uint32_t*>(c.v);
@@ -189,22 +96,10 @@ __global__ void __launch_bounds__(ra::THREADS)
     const int kg = BITS == 16 ? 0 : c4 * (HD / 4) / c.gs;  // this lane's group of a key row
     const int vg = BITS == 16 ? 0 : r8 * (HD / 8) / c.gs;  // and of a value row
 
-    while (u < u_hi) {
-        const Seq s = seq_of(a, b, G, ROWS);
-        const long long seq_units = static_cast<long long>(s.chunks) * s.tiles * Hkv;
-        if (u >= start + seq_units) {
-            start += seq_units;
-            ++b;
-            continue;
-        }
-        // the item: kv head fastest outside the tiles, so that neighbouring shares read
-        // neighbouring parts of the same pages
-        const int item = static_cast<int>((u - start) / s.tiles);
-        const int t0 = static_cast<int>((u - start) % s.tiles);
-        const int t1 = static_cast<int>(min(static_cast<long long>(s.tiles), t0 + (u_hi - u)));
-        const int g = item % Hkv, chunk = item / Hkv;
-        const int row_lo = chunk * ROWS, R = s.n * G;
-        const int base = s.L - s.n;  // keys before it are seen by every row
+    for (; w.next(a); w.advance()) {
+        const Seq& s = w.s;
+        const int g = w.g, row_lo = w.rr0, t0 = w.t0, t1 = w.t1, b = w.b, R = s.n * G;
+        const int base = w.base(), kend = w.kend(a), full = min(max(base, 0), kend);
         const int32_t* bt = a.table + static_cast<size_t>(b) * a.max_blocks;
 
         // Queries: lane (row r8 of the n-tile, quarter c4) holds its quarter's dims in the
@@ -215,19 +110,19 @@ __global__ void __launch_bounds__(ra::THREADS)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int rr = row_lo + 8 * nt + r8;
-            uint32_t w[HD / 8];
+            uint32_t qw[HD / 8];
 #pragma unroll
-            for (int i = 0; i < HD / 8; ++i) w[i] = 0u;
+            for (int i = 0; i < HD / 8; ++i) qw[i] = 0u;
             if (rr < R)
                 ldw(reinterpret_cast<const uint32_t*>(
                         q + (static_cast<size_t>(s.row0 + rr / G) * a.Hq + g * G + rr % G) * HD +
                         c4 * (HD / 4)),
-                    w);
+                    qw);
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
                 const int da = pair_dim<BITS>(i, 0), db = pair_dim<BITS>(i, 1);
                 bq[nt][i / 2][i % 2] =
-                    prmt(w[da / 2], w[db / 2], (da % 2 ? 0x32u : 0x10u) | (db % 2 ? 0x7600u : 0x5400u));
+                    prmt(qw[da / 2], qw[db / 2], (da % 2 ? 0x32u : 0x10u) | (db % 2 ? 0x7600u : 0x5400u));
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -237,11 +132,6 @@ __global__ void __launch_bounds__(ra::THREADS)
                 if (a.mask) vis[nt][e] = rc < R ? static_cast<unsigned long long>(a.mask[s.row0 + rc / G]) : 0ull;
             }
         }
-        // keys the chunk can see: with a causal mask, those up to its last row
-        const int last = min(R, row_lo + ROWS) - 1;
-        const int kend = max(0, a.mask ? s.L : min(s.L, base + last / G + 1));
-        const int full = min(max(base, 0), kend);  // keys every row sees
-
         float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -416,20 +306,21 @@ __global__ void __launch_bounds__(ra::THREADS)
                 }
             }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == s.tiles;
-        const size_t slot = (2 * static_cast<size_t>(blockIdx.x) + (u == u_lo ? 0 : 1)) * ROWS;
+        const bool whole = w.whole();
+        if (!whole && t0 == 0) mine = w.cut();
+        const size_t slot = static_cast<size_t>(w.slot()) * ROWS;
         for (int i = tid; i < ROWS * HD / 2; i += THREADS) {
             const int row = i / (HD / 2), d = 2 * (i % (HD / 2)), rr = row_lo + row;
             if (rr >= R) continue;
             float M = -INFINITY, den = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) M = fmaxf(M, wm[w][row]);
+            for (int i = 0; i < WARPS; ++i) M = fmaxf(M, wm[i][row]);
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float f = wm[w][row] == -INFINITY ? 0.f : exp2f(wm[w][row] - M);
-                den = fmaf(f, wl[w][row], den);
-                x = fmaf(f, wo[w][row][d], x);
-                y = fmaf(f, wo[w][row][d + 1], y);
+            for (int i = 0; i < WARPS; ++i) {
+                const float f = wm[i][row] == -INFINITY ? 0.f : exp2f(wm[i][row] - M);
+                den = fmaf(f, wl[i][row], den);
+                x = fmaf(f, wo[i][row][d], x);
+                y = fmaf(f, wo[i][row][d + 1], y);
             }
             if (whole) {
                 const float inv = M == -INFINITY ? 0.f : 1.0f / den;
@@ -441,127 +332,149 @@ __global__ void __launch_bounds__(ra::THREADS)
             }
         }
         __syncthreads();  // the shared results are read before the next item writes its own
-        u += t1 - t0;
     }
+    if (tid == 0) p.cut[blockIdx.x] = mine;
 }
 
-// Joins the parts of the items that were shared among CTAs: block (item of the whole
-// batch, row of its chunk), thread = dimension. Parts are taken in order of keys.
+// Joins the parts of the items that several CTAs took: block (CTA that began one, group of
+// 32 rows), warp = row, lane = HD / 32 dimensions. Parts are taken in order of keys.
 template <typename T, int HD, int ROWS>
-__global__ void __launch_bounds__(ra::THREADS)
-    attn_combine_kernel(const __grid_constant__ ra::Params p) {
+__global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant__ ra::Params p) {
     using namespace ra;
-    __shared__ long long pref[THREADS + 1];
+    constexpr int DPL = HD / 32;
     pdl_launch_dependents();
     pdl_wait();
+    const Cut c = p.cut[blockIdx.x];
     const RowsArgs& a = p.a;
-    const int Hkv = p.c.Hkv, G = a.Hq / Hkv;
-    const Units un = scan_units(a, Hkv, G, ROWS, pref);
-    const int P = static_cast<int>(min(static_cast<long long>(p.parts), un.total));
-    // an item that was cut holds some CTA's first or last unit: block (boundary i, row)
-    // takes the item that unit u_lo(i) lies inside of, if boundary i is its first
-    const int i = blockIdx.x + 1;
-    if (i >= P) return;
-    const long long x = un.total * i / P;
-    long long start;
-    const int b = find_seq(a, Hkv, G, ROWS, pref, un.per, x, start);
-    const Seq s = seq_of(a, b, G, ROWS);
-    const int item = static_cast<int>((x - start) / s.tiles);
-    const long long u0 = start + static_cast<long long>(item) * s.tiles;
-    if (x == u0) return;                     // the boundary is the item's own beginning
-    if (un.total * (i - 1) / P > u0) return; // an earlier boundary cuts the same item
-    const int g = item % Hkv, rr = item / Hkv * ROWS + static_cast<int>(blockIdx.y);
-    if (rr >= s.n * G) return;
-    const int first = owner(u0, un.total, P), lastc = owner(u0 + s.tiles - 1, un.total, P);
-    const int d = threadIdx.x;
-    float M = -INFINITY, den = 0.f, acc = 0.f;
+    const int G = a.Hq / p.c.Hkv, lane = threadIdx.x & 31;
+    const int end = min(c.rows, static_cast<int>(blockIdx.y + 1) * 32);
+    for (int r = blockIdx.y * 32 + (threadIdx.x >> 5); r < end; r += 8) {
+        float M = -INFINITY, den = 0.f, acc[DPL];
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
 #pragma unroll 4
-    for (int k = first; k <= lastc; ++k) {
-        const size_t slot = (2 * static_cast<size_t>(k) + (un.total * k / P >= u0 ? 0 : 1)) * ROWS +
-                            blockIdx.y;
-        const float2 ml = p.part_ml[slot];
-        const float v = d < HD ? p.part_o[slot * HD + d] : 0.f;
-        const float Mn = fmaxf(M, ml.x);
-        const float co = M == -INFINITY ? 0.f : exp2f(M - Mn);
-        const float cn = ml.x == -INFINITY ? 0.f : exp2f(ml.x - Mn);
-        den = fmaf(cn, ml.y, den * co);
-        acc = fmaf(cn, v, acc * co);
-        M = Mn;
+        for (int k = blockIdx.x; k <= c.last; ++k) {
+            const size_t at = static_cast<size_t>(k == blockIdx.x ? c.slot : 2 * k) * ROWS + r;
+            const float2 ml = __ldcg(&p.part_ml[at]);
+            float v[DPL];
+            if constexpr (DPL == 4) {
+                const float4 t = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD) + lane);
+                v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+            } else {
+                const float2 t = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * HD) + lane);
+                v[0] = t.x; v[1] = t.y;
+            }
+            const float Mn = fmaxf(M, ml.x);
+            const float co = M == -INFINITY ? 0.f : exp2f(M - Mn);
+            const float cn = ml.x == -INFINITY ? 0.f : exp2f(ml.x - Mn);
+            den = fmaf(cn, ml.y, den * co);
+#pragma unroll
+            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(cn, v[e], acc[e] * co);
+            M = Mn;
+        }
+        const float inv = M == -INFINITY ? 0.f : 1.0f / den;
+        const int rr = c.rr0 + r;
+        T* dst = static_cast<T*>(a.out) +
+                 (static_cast<size_t>(c.row0 + rr / G) * a.Hq + c.g * G + rr % G) * HD + lane * DPL;
+        if constexpr (DPL == 4)
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pk_round<T>(acc[0] * inv, acc[1] * inv),
+                                                        pk_round<T>(acc[2] * inv, acc[3] * inv));
+        else
+            *reinterpret_cast<uint32_t*>(dst) = pk_round<T>(acc[0] * inv, acc[1] * inv);
     }
-    if (d < HD)
-        static_cast<T*>(a.out)[(static_cast<size_t>(s.row0 + rr / G) * a.Hq + g * G + rr % G) * HD + d] =
-            Elem<T>::from_f(M == -INFINITY ? 0.f : acc / den);
 }
 
 namespace {
 
-// Query rows per chunk: a decode step's heads fit one n-tile of eight.
-int n_tiles(const KvCache& c, const RowsArgs& a) { return a.max_q * (a.Hq / c.Hkv) <= 8 ? 1 : 2; }
-
-// CTAs the units are shared out to: what the GPU holds at once (four CTAs of four warps
-// per SM with one n-tile, two with two), at most one per unit.
-int parts_of(const KvCache& c, const RowsArgs& a) {
-    const int nt = n_tiles(c, a), rows = 8 * nt;
-    const long long chunks = (static_cast<long long>(a.max_q) * (a.Hq / c.Hkv) + rows - 1) / rows;
-    const long long tiles = (a.max_kv + ra::KT - 1) / ra::KT;
-    long long units = chunks * (tiles > 0 ? tiles : 1) * c.Hkv;
-    const long long most = 148LL * (nt == 1 ? 4 : 2);
-    if (units > most) return static_cast<int>(most);
-    units *= a.batch;
-    return static_cast<int>(units < most ? (units > 0 ? units : 1) : most);
+// How a call is run: eight rows to a chunk where a decode step's heads fit them, sixteen
+// up to there, and from then on 128 of them as the M rows of tcgen05 products.
+struct Plan {
+    bool tc;
+    int rows, kt, parts;
+};
+Plan plan_of(const KvCache& c, const RowsArgs& a) {
+    const long long r = static_cast<long long>(a.max_q) * (a.Hq / c.Hkv);
+    Plan p;
+    p.tc = r > 16;
+    p.rows = p.tc ? 128 : r > 8 ? 16 : 8;
+    p.kt = p.tc ? kRowsTcKeys : ra::KT;
+    // CTAs the units are shared out to: what the GPU holds at once, at most one per unit
+    const long long most = 148LL * (p.rows == 8 ? 4 : 2);
+    const long long tiles = (a.max_kv + p.kt - 1) / p.kt;
+    long long units = (r + p.rows - 1) / p.rows * (tiles > 0 ? tiles : 1) * c.Hkv;
+    units = units < most ? units * a.batch : most;
+    p.parts = static_cast<int>(units < 1 ? 1 : units < most ? units : most);
+    return p;
 }
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 template <typename T, int HD, int BITS>
-const void* rows_fn(int nt) {
-    return nt == 1 ? reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 1>)
-                   : reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 2>);
+const void* rows_fn(int rows) {
+    return rows == 8 ? reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 1>)
+                     : reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 2>);
 }
 template <typename T, int HD>
-const void* rows_fn(int bits, int nt) {
-    return bits == 16 ? rows_fn<T, HD, 16>(nt) : bits == 8 ? rows_fn<T, HD, 8>(nt) : rows_fn<T, HD, 4>(nt);
+const void* rows_fn(int bits, int rows) {
+    return bits == 16 ? rows_fn<T, HD, 16>(rows) : bits == 8 ? rows_fn<T, HD, 8>(rows)
+                                                             : rows_fn<T, HD, 4>(rows);
 }
-template <typename T>
-const void* combine_fn(int hd, int nt) {
-    if (hd == 128)
-        return nt == 1 ? reinterpret_cast<const void*>(&attn_combine_kernel<T, 128, 8>)
-                       : reinterpret_cast<const void*>(&attn_combine_kernel<T, 128, 16>);
-    return nt == 1 ? reinterpret_cast<const void*>(&attn_combine_kernel<T, 64, 8>)
-                   : reinterpret_cast<const void*>(&attn_combine_kernel<T, 64, 16>);
+template <typename T, int HD>
+const void* combine_fn(int rows) {
+    return rows == 8    ? reinterpret_cast<const void*>(&attn_combine_kernel<T, HD, 8>)
+           : rows == 16 ? reinterpret_cast<const void*>(&attn_combine_kernel<T, HD, 16>)
+                        : reinterpret_cast<const void*>(&attn_combine_kernel<T, HD, 128>);
 }
 
 }  // namespace
 
 size_t attn_rows_workspace(const KvCache& c, const RowsArgs& a) {
-    const size_t slots = 2 * static_cast<size_t>(parts_of(c, a)) * 8 * n_tiles(c, a);
-    return slots * (c.hd * sizeof(float) + sizeof(float2));
+    const Plan pl = plan_of(c, a);
+    const size_t rows = 2 * static_cast<size_t>(pl.parts) * pl.rows;
+    return round256(rows * c.hd * sizeof(float)) + round256(rows * sizeof(float2)) +
+           round256(pl.parts * sizeof(ra::Cut));
 }
 
 cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspace, bool overlap,
                              cudaStream_t st) {
-    const int nt = n_tiles(c, a), P = parts_of(c, a);
+    const Plan pl = plan_of(c, a);
+    const size_t rows = 2 * static_cast<size_t>(pl.parts) * pl.rows;
     ra::Params p;
     p.a = a;
     p.c = c;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.parts = P;
-    p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + 2 * static_cast<size_t>(P) * 8 * nt * c.hd);
+    p.parts = pl.parts;
+    char* ws = static_cast<char*>(workspace);
+    p.part_o = reinterpret_cast<float*>(ws);
+    ws += round256(rows * c.hd * sizeof(float));
+    p.part_ml = reinterpret_cast<float2*>(ws);
+    ws += round256(rows * sizeof(float2));
+    p.cut = reinterpret_cast<ra::Cut*>(ws);
     void* args[] = {&p};
-    const bool bf = c.dtype == kBF16;
-    const void* f = bf ? (c.hd == 128 ? rows_fn<__nv_bfloat16, 128>(c.bits, nt)
-                                      : rows_fn<__nv_bfloat16, 64>(c.bits, nt))
-                       : (c.hd == 128 ? rows_fn<__half, 128>(c.bits, nt)
-                                      : rows_fn<__half, 64>(c.bits, nt));
-    static PerDevice cfg[24];
-    const int which = (((bf ? 0 : 1) * 2 + (c.hd == 128 ? 0 : 1)) * 3 +
-                       (c.bits == 16 ? 0 : c.bits == 8 ? 1 : 2)) * 2 + nt - 1;
-    cudaError_t e = launch_ex(f, cfg[which], dim3(P), dim3(ra::THREADS), 0, st, overlap, args);
-    if (e != cudaSuccess || P == 1) return e;
-    const void* fc = bf ? combine_fn<__nv_bfloat16>(c.hd, nt) : combine_fn<__half>(c.hd, nt);
-    static PerDevice cfgc[8];
+    const bool bf = c.dtype == kBF16, big = c.hd == 128;
+    const int variant = ((bf ? 0 : 1) * 2 + (big ? 0 : 1)) * 3 + (c.bits == 16 ? 0 : c.bits == 8 ? 1 : 2);
+    const int size = pl.rows == 8 ? 0 : pl.rows == 16 ? 1 : 2;
+    static PerDevice cfg[36];
+    cudaError_t e;
+    if (pl.tc) {
+        e = launch_ex(rows_tc_fn(c.dtype, c.hd, c.bits), cfg[variant * 3 + size], dim3(pl.parts),
+                      dim3(kRowsTcThreads), rows_tc_smem(c.hd), st, overlap, args);
+    } else {
+        const void* f = bf ? (big ? rows_fn<__nv_bfloat16, 128>(c.bits, pl.rows)
+                                  : rows_fn<__nv_bfloat16, 64>(c.bits, pl.rows))
+                           : (big ? rows_fn<__half, 128>(c.bits, pl.rows)
+                                  : rows_fn<__half, 64>(c.bits, pl.rows));
+        e = launch_ex(f, cfg[variant * 3 + size], dim3(pl.parts), dim3(ra::THREADS), 0, st, overlap,
+                      args);
+    }
+    if (e != cudaSuccess || pl.parts == 1) return e;
+    const void* fc = bf ? (big ? combine_fn<__nv_bfloat16, 128>(pl.rows)
+                               : combine_fn<__nv_bfloat16, 64>(pl.rows))
+                        : (big ? combine_fn<__half, 128>(pl.rows) : combine_fn<__half, 64>(pl.rows));
+    static PerDevice cfgc[12];
     // (its launch may begin while the parts are computed; it waits for them all)
-    return launch_ex(fc, cfgc[((bf ? 0 : 1) * 2 + (c.hd == 128 ? 0 : 1)) * 2 + nt - 1],
-                     dim3(P - 1, 8 * nt), dim3(ra::THREADS), 0, st, true, args);
+    return launch_ex(fc, cfgc[(variant / 3) * 3 + size], dim3(pl.parts - 1, (pl.rows + 31) / 32),
+                     dim3(256), 0, st, true, args);
 }
 
 }  // namespace mlxq

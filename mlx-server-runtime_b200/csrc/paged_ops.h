@@ -49,4 +49,11 @@ size_t attn_rows_workspace(const KvCache& c, const RowsArgs& a);
 cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspace, bool overlap,
                              cudaStream_t st);
 
+// The tcgen05 form of the attention kernel (paged_attn_tc.cu): 128 query rows and kRowsTcKeys
+// keys to a tile.
+constexpr int kRowsTcKeys = 128, kRowsTcThreads = 288;
+const void* rows_tc_fn(int dtype, int hd, int bits);
+size_t rows_tc_smem(int hd);
+cudaError_t rows_tc_read_error(int* code);
+
 }  // namespace mlxq

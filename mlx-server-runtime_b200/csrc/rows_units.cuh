@@ -1,0 +1,179 @@
+// How attention over pages shares its work out: the query rows of every (sequence, kv head)
+// in chunks, each chunk's keys in tiles, and the tiles of all (sequence, chunk, kv head)
+// items as one sequence of units that the CTAs take in equal contiguous runs. And how the
+// parts of an item that several CTAs computed are joined.
+#pragma once
+
+#include "common.cuh"
+#include "paged_ops.h"
+
+namespace mlxq {
+namespace ra {
+
+// An item whose tiles several CTAs took, recorded by the CTA that took the first of them:
+// its partial results are in that CTA's slot `slot`, then in slot 0 of the CTAs up to
+// `last`, in order of keys.
+struct Cut {
+    int rows;   // rows of the chunk (0: this CTA began no such item)
+    int slot, last;
+    int row0, rr0, g;  // the sequence's first row of q, the chunk's first row, the kv head
+};
+
+struct Params {
+    RowsArgs a;
+    KvCache c;
+    float scale_log2;
+    float* part_o;    // [2 P][ROWS][HD] unnormalised outputs
+    float2* part_ml;  // [2 P][ROWS] maximum (base 2) and sum
+    Cut* cut;         // [P]
+    int parts;        // P: CTAs the units are shared out to
+};
+
+// One sequence's place in the batch, with everything a bad length or offset could do bounded.
+struct Seq {
+    int row0, n, L, chunks, tiles;
+};
+template <int KT>
+__device__ __forceinline__ Seq seq_of(const RowsArgs& a, int b, int G, int rows) {
+    Seq s;
+    int lo = b, hi = b + 1;
+    if (a.cu_q) {
+        lo = a.cu_q[b];
+        hi = a.cu_q[b + 1];
+    }
+    s.row0 = max(0, min(lo, a.total));
+    s.n = max(0, min(min(hi, a.total) - s.row0, a.max_q));
+    s.L = max(0, min(a.kv_lens[b], a.max_kv));
+    s.chunks = (s.n * G + rows - 1) / rows;
+    s.tiles = max(1, (s.L + KT - 1) / KT);  // a sequence without keys still writes its zeros
+    return s;
+}
+
+// Prefix sums of the batch's units, thread i < SCAN over a run of sequences. Every thread of
+// the CTA calls it.
+constexpr int SCAN = 128;
+struct Units {
+    long long total;
+    int per;  // sequences per scanning thread
+};
+template <int KT>
+__device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, int rows,
+                                            long long* pref /* shared [SCAN + 1] */) {
+    __shared__ long long wsum[SCAN / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    Units u;
+    u.per = (a.batch + SCAN - 1) / SCAN;
+    long long inc = 0;
+    if (tid < SCAN) {
+        for (int b = tid * u.per; b < min(a.batch, (tid + 1) * u.per); ++b) {
+            const Seq s = seq_of<KT>(a, b, G, rows);
+            inc += static_cast<long long>(s.chunks) * s.tiles * Hkv;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) wsum[warp] = inc;
+    }
+    __syncthreads();
+    if (tid < SCAN) {
+        for (int w = 0; w < warp; ++w) inc += wsum[w];
+        pref[tid + 1] = inc;
+        if (tid == 0) pref[0] = 0;
+    }
+    __syncthreads();
+    u.total = pref[SCAN];
+    return u;
+}
+
+// A CTA's run of units as segments, each a range of tiles of one item.
+template <int KT, int ROWS>
+struct Walk {
+    long long u, u_lo, u_hi, start, total;
+    int b, G, Hkv, P;
+    // the segment
+    Seq s;
+    int g, rr0, t0, t1;
+    long long item_u0;
+
+    __device__ __forceinline__ void begin(const RowsArgs& a, int Hkv_, const Units& un, int parts,
+                                          const long long* pref) {
+        Hkv = Hkv_;
+        G = a.Hq / Hkv;
+        total = un.total;
+        P = static_cast<int>(min(static_cast<long long>(parts), total));  // no share is empty
+        u = u_lo = u_hi = 0;
+        if (static_cast<int>(blockIdx.x) >= P) return;
+        u = u_lo = total * blockIdx.x / P;
+        u_hi = total * (blockIdx.x + 1) / P;
+        int lo = 0, hi = SCAN - 1;  // the last run of sequences that begins at or before u
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (pref[mid] <= u) lo = mid;
+            else hi = mid - 1;
+        }
+        start = pref[lo];
+        b = lo * un.per;
+    }
+    // Steps to the segment at u; false at the end of the run.
+    __device__ __forceinline__ bool next(const RowsArgs& a) {
+        while (u < u_hi) {
+            s = seq_of<KT>(a, b, G, ROWS);
+            const long long n = static_cast<long long>(s.chunks) * s.tiles * Hkv;
+            if (u >= start + n) {
+                start += n;
+                ++b;
+                continue;
+            }
+            // kv head fastest outside the tiles: neighbouring runs read neighbouring parts
+            // of the same pages
+            const int item = static_cast<int>((u - start) / s.tiles);
+            t0 = static_cast<int>((u - start) % s.tiles);
+            t1 = static_cast<int>(min(static_cast<long long>(s.tiles), t0 + (u_hi - u)));
+            item_u0 = u - t0;
+            g = item % Hkv;
+            rr0 = item / Hkv * ROWS;
+            return true;
+        }
+        return false;
+    }
+    __device__ __forceinline__ void advance() { u += t1 - t0; }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == s.tiles; }
+    __device__ __forceinline__ int slot() const { return 2 * blockIdx.x + (u == u_lo ? 0 : 1); }
+    // keys the chunk can see (with a causal mask, those up to its last row), of them the
+    // ones every row sees, and the position of new token 0
+    __device__ __forceinline__ int base() const { return s.L - s.n; }
+    __device__ __forceinline__ int kend(const RowsArgs& a) const {
+        const int last = min(s.n * G, rr0 + ROWS) - 1;
+        return max(0, a.mask ? s.L : min(s.L, base() + last / G + 1));
+    }
+    // The CTA that owns unit x of the run of all.
+    __device__ __forceinline__ int owner(long long x) const {
+        return static_cast<int>(((x + 1) * P - 1) / total);
+    }
+    __device__ __forceinline__ Cut cut() const {
+        Cut c;
+        c.rows = min(s.n * G - rr0, ROWS);
+        c.slot = slot();
+        c.last = owner(item_u0 + s.tiles - 1);
+        c.row0 = s.row0;
+        c.rr0 = rr0;
+        c.g = g;
+        return c;
+    }
+};
+
+// Rows behind the last sequence are zero.
+__device__ __forceinline__ void zero_tail(const RowsArgs& a, int HD, int threads) {
+    if (!a.cu_q) return;
+    const long long row = static_cast<long long>(a.Hq) * HD / 8;
+    const int end = max(0, min(a.cu_q[a.batch], a.total));
+    uint4* o = static_cast<uint4*>(a.out);
+    for (long long i = end * row + blockIdx.x * threads + threadIdx.x; i < a.total * row;
+         i += static_cast<long long>(gridDim.x) * threads)
+        o[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
+}  // namespace ra
+}  // namespace mlxq
