@@ -12,7 +12,7 @@
 //               memory as it lies (key rows, dimensions contiguous)
 // Warps 0-3 hold a tensor-memory lane quarter each and do the softmax and the epilogue;
 // warps 4-7 bring keys and values into shared memory, dequantised once per tile on the way
-// (16-bit rows by cp.async); one thread of warp 8 issues the products. The chain S ->
+// (16-bit rows by cp.async), and a thread of warp 4 issues the products between its loads. The chain S ->
 // softmax -> P V of a CTA is serial; two CTAs share an SM (96 KB of shared memory and 256
 // columns each), so one's products run under the other's softmax, and a tile's loads have
 // most of the chain to land in (K is free once S is done, V once P V is).
@@ -34,7 +34,7 @@ __device__ int g_rows_tc_error;  // 0, or the first error code a kernel recorded
 
 namespace rt {
 constexpr int ROWS = 128, KT = kRowsTcKeys, THREADS = kRowsTcThreads;
-constexpr int WARP_LOAD0 = 4, WARP_MMA = 8;
+constexpr int WARP_LOAD0 = 4;  // the loads; the first of these warps also issues the products
 constexpr uint32_t kCols = 256;   // tensor memory: S (and P) from 0, O from 128
 constexpr uint32_t kOCol = 128;
 constexpr uint32_t kParkNs = 2000, kParkLimit = 1u << 20;  // ~2 s
@@ -48,6 +48,31 @@ constexpr int tile_bytes() { return KT * HD * 2; }
 template <int BITS>
 __host__ __device__ constexpr int staged_dim(int x) {
     return BITS == 16 ? x : pair_dim<BITS>(x / 2, x % 2);
+}
+
+// Pairs of 32-bit floats in one register pair: one instruction for two lanes of work.
+__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {  // 2^x, results below 2^-126 as zero
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+    return r;
 }
 }  // namespace rt
 
@@ -74,7 +99,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     uint8_t *qs = smem, *ks = smem + ROWS * HD * 2, *vs = ks + TB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_launch_dependents();
-    if (warp == WARP_MMA) {
+    if (warp == WARP_LOAD0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(
                          smem_u32(&tmem_slot)),
                      "r"(kCols));
@@ -113,9 +138,10 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     // tiles of the segment that hold keys its rows can see
     auto tile_end = [&]() { return min(w.t1, (w.kend(a) + KT - 1) / KT); };
 
-    if (warp >= WARP_LOAD0 && warp < WARP_MMA) {
-        // ------------------------------ loads ---------------------------------------
+    if (warp >= WARP_LOAD0) {
+        // ------------------------------ loads and products ---------------------------
         const int lw = warp - WARP_LOAD0;   // this warp's 32 rows of every tile
+        const bool issuer = lw == 0 && lane == 0;
         const int c0 = lane % LPR, r0 = lane / LPR;
         const int grp = BITS == 16 ? 0 : c0 * (128 / BITS) / c.gs;
         const int ng = BITS == 16 ? 1 : HD / c.gs;
@@ -124,8 +150,41 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             return static_cast<uint32_t>((ch / 8) * (KT * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4));
         };
         const bool neg = p.scale_log2 < 0.f;  // the sign of the scale goes into the queries
-        uint32_t it = 0;                      // tiles staged so far
-        bool ok = true;
+        const uint64_t qd = sw128_kmajor_desc(smem_u32(qs)), kd = sw128_kmajor_desc(smem_u32(ks));
+        const uint64_t vd = sw128_mnmajor_desc(smem_u32(vs), KT * 128);
+        uint32_t it = 0;     // tiles so far
+        bool ok = true, acc = false;  // acc: the tile before was not its item's first here
+        auto spin = [&](uint64_t* bar, uint32_t parity) -> bool {
+            // (the issuing thread polls without parking: it wakes fastest)
+            if (!s_abort && mbar_wait_bounded(smem_u32(bar), parity, kSpinLimit)) return true;
+            atomicCAS(&g_rows_tc_error, 0, kErrTimeout);
+            s_abort = 1;
+            return false;
+        };
+        auto issue_s = [&](uint32_t i) {
+            if (!spin(&k_full, i & 1)) return;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes of a half
+                const uint64_t off = static_cast<uint64_t>((j / 4) * (KT * 128 / 16) + (j % 4) * 2);
+                umma_f16_ss(tmem, qd + off, kd + off, IDESC_S, j > 0 ? 1u : 0u);
+            }
+            umma_commit(smem_u32(&s_full));
+        };
+        auto issue_pv = [&](uint32_t i, bool accumulate) {
+            if (!spin(&v_full, i & 1) || !spin(&p_full, i & 1)) return;
+            tc_fence_after();
+#pragma unroll
+            for (int j = 0; j < KT / 16; ++j)  // 16 keys: 8 columns of P, 2 KB of V
+                umma_f16_ts(tmem + kOCol, tmem + 8 * j, vd + j * (2048 / 16), IDESC_O,
+                            (accumulate || j > 0) ? 1u : 0u);
+            umma_commit(smem_u32(&pv_done));
+        };
+        auto arrive = [&](uint64_t* bar) {  // this warp's rows are in shared memory
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(bar));
+        };
         for (; ok && w.next(a); w.advance()) {
             const Seq& s = w.s;
             const int kend = w.kend(a), te = tile_end(), R = s.n * G;
@@ -139,35 +198,38 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
                     if (pid >= 0 && pid < c.pages)
                         mine = (static_cast<long long>(pid) * c.page + key % c.page) * Hkv + w.g;
                 }
-                uint4 kr[BITS == 16 ? 1 : LPR], vr[BITS == 16 ? 1 : LPR];
-                uint32_t ksb[LPR], vsb[LPR];
+                // Quantised rows of the tile, all loads in flight together
+                constexpr int NL = BITS == 16 ? 1 : LPR;
+                uint4 kr[NL], vr[NL];
+                uint16_t ksr[NL], kbr[NL], vsr[NL], vbr[NL];
+                uint32_t there = 0;
                 if constexpr (BITS != 16) {
 #pragma unroll
                     for (int i = 0; i < LPR; ++i) {
-                        const long long row = __shfl_sync(0xffffffffu, mine, i * RPI + r0);
-                        kr[i] = vr[i] = make_uint4(0u, 0u, 0u, 0u);
-                        ksb[i] = vsb[i] = 0u;  // a key that is not there: zeros
-                        if (row >= 0) {
-                            kr[i] = *reinterpret_cast<const uint4*>(
-                                static_cast<const uint32_t*>(c.k) + row * RW + c0 * 4);
-                            vr[i] = *reinterpret_cast<const uint4*>(
-                                static_cast<const uint32_t*>(c.v) + row * RW + c0 * 4);
-                            const long long g = row * ng + grp;
-                            ksb[i] = static_cast<const uint16_t*>(c.ks)[g] |
-                                     static_cast<uint32_t>(static_cast<const uint16_t*>(c.kb)[g]) << 16;
-                            vsb[i] = static_cast<const uint16_t*>(c.vs)[g] |
-                                     static_cast<uint32_t>(static_cast<const uint16_t*>(c.vb)[g]) << 16;
-                        }
+                        const long long own = __shfl_sync(0xffffffffu, mine, i * RPI + r0);
+                        const long long row = own < 0 ? 0 : own;
+                        there |= own < 0 ? 0u : 1u << i;
+                        kr[i] = __ldg(reinterpret_cast<const uint4*>(
+                            static_cast<const uint32_t*>(c.k) + row * RW + c0 * 4));
+                        vr[i] = __ldg(reinterpret_cast<const uint4*>(
+                            static_cast<const uint32_t*>(c.v) + row * RW + c0 * 4));
+                        const long long g = row * ng + grp;
+                        ksr[i] = static_cast<const uint16_t*>(c.ks)[g];
+                        kbr[i] = static_cast<const uint16_t*>(c.kb)[g];
+                        vsr[i] = static_cast<const uint16_t*>(c.vs)[g];
+                        vbr[i] = static_cast<const uint16_t*>(c.vb)[g];
                     }
                 }
                 // Stages the loaded rows of a tile: 16 bytes of codes become CPU chunks. Lanes
                 // of the upper half take theirs in another order, so that the eight lanes of
-                // a store phase meet eight different bank groups.
-                auto stage = [&](uint8_t* dst, const uint4* raw, const uint32_t* sb) {
+                // a store phase meet eight different bank groups. A key that is not there is
+                // zeros (its stale values must not meet a probability of zero).
+                auto stage = [&](uint8_t* dst, const uint4* raw, const uint16_t* sr, const uint16_t* br) {
 #pragma unroll
-                    for (int i = 0; i < LPR; ++i) {
+                    for (int i = 0; i < NL; ++i) {
                         const int r = lw * 32 + i * RPI + r0;
-                        const uint32_t s2 = pk_splat(sb[i]), b2 = prmt(sb[i], 0u, 0x3232u);
+                        const bool in = there >> i & 1;
+                        const uint32_t s2 = in ? pk_splat(sr[i]) : 0u, b2 = in ? pk_splat(br[i]) : 0u;
                         const bool up = HD == 128 && c0 >= LPR / 2;
                         uint32_t wd[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                         constexpr int flip = CPU / 2;  // chunks exchanged: q ^ flip
@@ -203,98 +265,76 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
                     break;
                 }
                 if (tile == w.t0) {
-                    constexpr int QL = HD / 8;  // lanes of a query row
-                    for (int i = 0; i < QL; ++i) {
-                        const int r = lw * 32 + i * (32 / QL) + lane / QL, rr = w.rr0 + r;
-                        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                        if (rr < R)
-                            v = *reinterpret_cast<const uint4*>(
-                                static_cast<const T*>(a.q) +
-                                (static_cast<size_t>(s.row0 + rr / G) * a.Hq + w.g * G + rr % G) * HD +
-                                (lane % QL) * 8);
-                        if (neg) {
-                            v.x ^= 0x80008000u; v.y ^= 0x80008000u;
-                            v.z ^= 0x80008000u; v.w ^= 0x80008000u;
-                        }
-                        const uint32_t wd[4] = {v.x, v.y, v.z, v.w};
-                        uint32_t o[4];
+                    constexpr int QL = HD / 8, QB = 8;  // lanes of a query row; loads at once
+#pragma unroll 1
+                    for (int i0 = 0; i0 < QL; i0 += QB) {
+                        uint4 v[QB];
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            constexpr uint32_t lo = 0x10u, hi = 0x32u;
-                            const int da = staged_dim<BITS>(2 * x), db = staged_dim<BITS>(2 * x + 1);
-                            o[x] = prmt(wd[da / 2], wd[db / 2],
-                                        (da % 2 ? hi : lo) | ((db % 2 ? hi : lo) + 0x44u) << 8);
+                        for (int i = 0; i < QB; ++i) {
+                            const int rr = w.rr0 + lw * 32 + (i0 + i) * (32 / QL) + lane / QL;
+                            v[i] = make_uint4(0u, 0u, 0u, 0u);
+                            if (rr < R)
+                                v[i] = *reinterpret_cast<const uint4*>(
+                                    static_cast<const T*>(a.q) +
+                                    (static_cast<size_t>(s.row0 + rr / G) * a.Hq + w.g * G + rr % G) * HD +
+                                    (lane % QL) * 8);
                         }
-                        *reinterpret_cast<uint4*>(qs + at(r, lane % QL)) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+                        for (int i = 0; i < QB; ++i) {
+                            const uint32_t flip = neg ? 0x80008000u : 0u;
+                            const uint32_t wd[4] = {v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip};
+                            uint32_t o[4];
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const int da = staged_dim<BITS>(2 * x), db = staged_dim<BITS>(2 * x + 1);
+                                o[x] = prmt(wd[da / 2], wd[db / 2],
+                                            (da % 2 ? 0x32u : 0x10u) | (db % 2 ? 0x7600u : 0x5400u));
+                            }
+                            *reinterpret_cast<uint4*>(
+                                qs + at(lw * 32 + (i0 + i) * (32 / QL) + lane / QL, lane % QL)) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
+                        }
                     }
                 }
-                if constexpr (BITS == 16) copy(ks, c.k);
-                else {
-                    stage(ks, kr, ksb);
-                    fence_async_smem();
+                // K of this tile goes in while the rows' softmax of the one before runs, then
+                // that one's P V and this one's S are issued, then V of this tile goes in
+                if constexpr (BITS == 16) {
+                    copy(ks, c.k);
+                    if (it > 0) {
+                        cp_async_wait<1>();
+                        arrive(&v_full);
+                        if (issuer) issue_pv(it - 1, acc);
+                        __syncwarp();
+                    }
+                    cp_async_wait<0>();
+                    arrive(&k_full);
+                } else {
+                    stage(ks, kr, ksr, kbr);
+                    arrive(&k_full);
+                    if (issuer && it > 0) issue_pv(it - 1, acc);
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&k_full));
                 }
+                if (issuer) issue_s(it);
+                __syncwarp();
+                acc = tile > w.t0;
                 if (it > 0 && !wait(&pv_done, (it - 1) & 1)) {
                     ok = false;
                     break;
                 }
                 if constexpr (BITS == 16) {
                     copy(vs, c.v);
-                    cp_async_wait<1>();
-                    fence_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&k_full));
-                    cp_async_wait<0>();
                 } else {
-                    stage(vs, vr, vsb);
+                    stage(vs, vr, vsr, vbr);
+                    arrive(&v_full);
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&v_full));
             }
         }
-        cp_async_wait<0>();
-    } else if (warp == WARP_MMA) {
-        // ------------------------------ products ------------------------------------
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            auto spin = [&](uint64_t* bar, uint32_t parity) -> bool {
-                // (polls without parking: it wakes fastest)
-                if (!s_abort && mbar_wait_bounded(smem_u32(bar), parity, kSpinLimit)) return true;
-                atomicCAS(&g_rows_tc_error, 0, kErrTimeout);
-                s_abort = 1;
-                return false;
-            };
-            const uint64_t qd = sw128_kmajor_desc(smem_u32(qs)), kd = sw128_kmajor_desc(smem_u32(ks));
-            const uint64_t vd = sw128_mnmajor_desc(smem_u32(vs), KT * 128);
-            for (; ok && w.next(a); w.advance()) {
-                const int te = tile_end();
-                for (int tile = w.t0; tile < te; ++tile, ++it) {
-                    if (!spin(&k_full, it & 1)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-#pragma unroll
-                    for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes of a half
-                        const uint64_t off = static_cast<uint64_t>((j / 4) * (KT * 128 / 16) + (j % 4) * 2);
-                        umma_f16_ss(tmem, qd + off, kd + off, IDESC_S, j > 0 ? 1u : 0u);
-                    }
-                    umma_commit(smem_u32(&s_full));
-                    if (!spin(&v_full, it & 1) || !spin(&p_full, it & 1)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-#pragma unroll
-                    for (int j = 0; j < KT / 16; ++j)  // 16 keys: 8 columns of P, 2 KB of V
-                        umma_f16_ts(tmem + kOCol, tmem + 8 * j, vd + j * (2048 / 16), IDESC_O,
-                                    (tile > w.t0 || j > 0) ? 1u : 0u);
-                    umma_commit(smem_u32(&pv_done));
-                }
-            }
+        if constexpr (BITS == 16) {
+            cp_async_wait<0>();
+            if (ok && it > 0) arrive(&v_full);
+        }
+        if (issuer) {
+            if (ok && it > 0) issue_pv(it - 1, acc);
             // every product issued has finished before tensor memory is freed
             umma_commit(smem_u32(&drained));
             mbar_wait_bounded(smem_u32(&drained), 0, kSpinLimit);
@@ -341,26 +381,36 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
                 }
                 tc_fence_after();
                 if (some) {
-                    auto seen = [&](int x) -> bool {  // key x of the tile
-                        const int key = k0 + x, j = key - base;
-                        return key < kend && (pages_ok >> (x / 8) & 1) &&
-                               (j < 0 || (a.mask ? j < 64 && (vis >> (j & 63) & 1) : j <= tok));
+                    // the keys of the tile's q-th 32 that this row sees, a bit each
+                    auto seen32 = [&](int q) -> uint32_t {
+                        const int kk = k0 + 32 * q, left = kend - kk, j0 = kk - base;
+                        uint32_t bits = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+                        bits &= ((pages_ok >> (4 * q) & 15u) * 0x00204081u & 0x01010101u) * 255u;
+                        if (j0 <= -32) return bits;
+                        if (a.mask)
+                            return bits & (j0 >= 64  ? 0u
+                                           : j0 >= 0 ? static_cast<uint32_t>(vis >> j0)
+                                                     : static_cast<uint32_t>(vis << -j0) | ((1u << -j0) - 1u));
+                        const int n = tok - j0 + 1;
+                        return bits & (n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u);
                     };
                     float mx = -INFINITY;
 #pragma unroll 1
                     for (int q = 0; q < KT / 32; ++q) {
                         uint32_t v[32];
                         tmem_ld32(t_s + q * 32, v);
-                        if (clean) {
-                            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                            for (int x = 0; x < 32; ++x) m4[x & 3] = fmaxf(m4[x & 3], __uint_as_float(v[x]));
-                            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
-                        } else {
+                        if (!clean) {
+                            const uint32_t bits = seen32(q);
 #pragma unroll
                             for (int x = 0; x < 32; ++x)
-                                mx = fmaxf(mx, seen(q * 32 + x) ? __uint_as_float(v[x]) : -INFINITY);
+                                v[x] = bits >> x & 1 ? v[x] : 0xff800000u;
                         }
+                        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2)
+                            m4[x / 2 & 3] = fmaxf(m4[x / 2 & 3],
+                                                  fmaxf(__uint_as_float(v[x]), __uint_as_float(v[x + 1])));
+                        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
                     }
                     mx = mx == -INFINITY ? mx : mx * scale;  // (a scale of zero keeps -inf)
                     if (__any_sync(0xffffffffu, mx - m > 8.f)) {
@@ -380,24 +430,37 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
                         }
                     }
                     const float mr = m == -INFINITY ? 0.f : m;
+                    const uint64_t scale2 = pack_f2(scale, scale), mr2 = pack_f2(-mr, -mr);
+                    uint64_t l2 = pack_f2(l, 0.f);
 #pragma unroll 1
                     for (int q = 0; q < KT / 32; ++q) {
                         uint32_t v[32], o[16];
                         tmem_ld32(t_s + q * 32, v);
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) {
-                            float e0 = exp2f(fmaf(__uint_as_float(v[x]), scale, -mr));
-                            float e1 = exp2f(fmaf(__uint_as_float(v[x + 1]), scale, -mr));
-                            if (!clean) {
-                                e0 = seen(q * 32 + x) ? e0 : 0.f;
-                                e1 = seen(q * 32 + x + 1) ? e1 : 0.f;
-                            }
-                            l += e0 + e1;
+                            float e0, e1;
+                            unpack_f2(fma_f2(pack_f2(__uint_as_float(v[x]), __uint_as_float(v[x + 1])),
+                                             scale2, mr2), e0, e1);
+                            v[x] = __float_as_uint(ex2(e0));
+                            v[x + 1] = __float_as_uint(ex2(e1));
+                        }
+                        if (!clean) {
+                            const uint32_t bits = seen32(q);
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) v[x] = bits >> x & 1 ? v[x] : 0u;
+                        }
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2) {
+                            const float e0 = __uint_as_float(v[x]), e1 = __uint_as_float(v[x + 1]);
+                            l2 = add_f2(l2, pack_f2(e0, e1));
                             o[x / 2] = pk_round<T>(e0, e1);
                         }
                         // (columns 16 q .. 16 q + 15 of S were read in this or an earlier step)
                         tmem_st16(t_s + q * 16, o);
                     }
+                    float la, lb;
+                    unpack_f2(l2, la, lb);
+                    l = la + lb;
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -446,7 +509,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == WARP_MMA) {
+    if (warp == WARP_LOAD0) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kCols));
     }

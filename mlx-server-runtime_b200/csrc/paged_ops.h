@@ -51,7 +51,7 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspac
 
 // The tcgen05 form of the attention kernel (paged_attn_tc.cu): 128 query rows and kRowsTcKeys
 // keys to a tile.
-constexpr int kRowsTcKeys = 128, kRowsTcThreads = 288;
+constexpr int kRowsTcKeys = 128, kRowsTcThreads = 256;
 const void* rows_tc_fn(int dtype, int hd, int bits);
 size_t rows_tc_smem(int hd);
 cudaError_t rows_tc_read_error(int* code);
