@@ -5,6 +5,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "paged_ops.h"
 
 namespace mlxq {
 
@@ -99,6 +100,35 @@ __device__ __forceinline__ uint32_t cross_pair(const uint32_t* wa, const uint32_
     } else {
         const uint32_t h = prmt(wa[i / 8], wb[i / 8], (i % 8) < 4 ? 0x5410u : 0x7632u);
         return pk_fma<T>(nibbles_pair<T>(h >> (4 * (i % 4))), s2, b2);
+    }
+}
+
+// Eight values of a pool: chunk `at` of eight elements of its rows.
+template <typename T, int BITS>
+__device__ __forceinline__ uint4 cache_chunk(const KvCache& c, bool is_v, size_t at) {
+    const void* data = is_v ? c.v : c.k;
+    if constexpr (BITS == 16) {
+        return static_cast<const uint4*>(data)[at];
+    } else {
+        uint32_t w[BITS / 4], p[4];
+        if constexpr (BITS == 8) {
+            const uint2 v = static_cast<const uint2*>(data)[at];
+            w[0] = v.x;
+            w[1] = v.y;
+        } else {
+            w[0] = static_cast<const uint32_t*>(data)[at];
+        }
+        const size_t g = at * 8 / c.gs;
+        const uint32_t s = pk_splat(static_cast<const uint16_t*>(is_v ? c.vs : c.ks)[g]);
+        const uint32_t b = pk_splat(static_cast<const uint16_t*>(is_v ? c.vb : c.kb)[g]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = row_pair<T, BITS>(w, j, s, b);
+        if constexpr (BITS == 8)  // pairs (0,2) (1,3) (4,6) (5,7)
+            return make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[0], p[1], 0x7632u),
+                              prmt(p[2], p[3], 0x5410u), prmt(p[2], p[3], 0x7632u));
+        // pairs (0,4) (1,5) (2,6) (3,7)
+        return make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u),
+                          prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
     }
 }
 

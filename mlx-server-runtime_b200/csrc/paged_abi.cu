@@ -38,6 +38,8 @@ int check_cache(const mlxq_kv_cache* c, int n_q_heads, const char* what, mlxq::K
                                           "query heads per kv head");
     if (c->num_pages <= 0 || c->num_pages > kIntMax / c->page_size)
         return fail(MLXQ_ERR_SHAPE, what, "num_pages must be positive, with fewer than 2^31 rows");
+    if (c->num_pages * c->page_size >= (1LL << 32) / c->n_kv_heads)
+        return fail(MLXQ_ERR_SHAPE, what, "a pool holds fewer than 2^32 rows of one head");
     if (!c->k || !c->v) return fail(MLXQ_ERR_NULL, what, "NULL cache pool");
     if (!aligned(c->k, 16) || !aligned(c->v, 16))
         return fail(MLXQ_ERR_ALIGN, what, "cache pools must be 16-byte aligned");
@@ -164,6 +166,9 @@ int mlxq_paged_attention_rows(const mlxq_kv_cache* cache, const void* q, const i
     a.batch = static_cast<int>(batch);
     a.Hq = n_q_heads;
     a.scale = scale;
+    a.tail = true;
+    if (!mlxq::attn_rows_countable(c, a))
+        return fail(MLXQ_ERR_SHAPE, what, "batch, query and key lengths are too large together");
     const size_t need = mlxq::attn_rows_workspace(c, a);
     if (need) {
         if (!workspace || workspace_bytes < need)

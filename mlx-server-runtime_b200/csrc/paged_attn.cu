@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(ra::THREADS)
     constexpr int VW = HD / 8 * BITS / 32;  // words of a value row per lane (an eighth)
     constexpr int RW = HD * BITS / 32;      // words of a row
     constexpr int MT = HD / 16;
-    __shared__ long long pref[THREADS + 1];
+    __shared__ int pref[SCAN + 1];
     __shared__ float wo[WARPS][ROWS][HD + 4];
     __shared__ float wm[WARPS][ROWS], wl[WARPS][ROWS];
     pdl_launch_dependents();
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(ra::THREADS)
 
     for (; w.next(a); w.advance()) {
         const Seq& s = w.s;
-        const int g = w.g, row_lo = w.rr0, t0 = w.t0, t1 = w.t1, b = w.b, R = s.n * G;
+        const int g = w.g, row_lo = w.rr0, t0 = w.t0, b = w.b, R = s.n * G;
         const int base = w.base(), kend = w.kend(a), full = min(max(base, 0), kend);
         const int32_t* bt = a.table + static_cast<size_t>(b) * a.max_blocks;
 
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(ra::THREADS)
                 }
             }
         };
-        const int te = min(t1, (kend + KT - 1) / KT);
+        const int te = w.tile_end(a);
         if (t0 < te) load(t0);
         for (int tile = t0; tile < te; ++tile) {
             const int k0 = tile * KT + warp * 16;
@@ -428,21 +428,43 @@ const void* combine_fn(int rows) {
 
 }  // namespace
 
+bool attn_rows_countable(const KvCache& c, const RowsArgs& a) {
+    const Plan pl = plan_of(c, a);
+    const long long r = static_cast<long long>(a.max_q) * (a.Hq / c.Hkv);
+    const double units = static_cast<double>((r + pl.rows - 1) / pl.rows) * c.Hkv * a.batch *
+                         (a.max_kv / pl.kt + 1);
+    return units < 2147483647.0;
+}
+
+namespace {
+
+// Sequences whose expanded rows are held at once: as many as 1 GiB takes, one at least.
+int group_of(const KvCache& c, const RowsArgs& a, const Plan& pl) {
+    if (!pl.tc || c.bits == 16) return a.batch;
+    const size_t each = rows_tc_expand_bytes(c, a);
+    const size_t n = each ? (size_t{1} << 30) / each : a.batch;
+    return static_cast<int>(n < 1 ? 1 : n < static_cast<size_t>(a.batch) ? n : a.batch);
+}
+
+}  // namespace
+
 size_t attn_rows_workspace(const KvCache& c, const RowsArgs& a) {
     const Plan pl = plan_of(c, a);
     const size_t rows = 2 * static_cast<size_t>(pl.parts) * pl.rows;
-    return round256(rows * c.hd * sizeof(float)) + round256(rows * sizeof(float2)) +
-           round256(pl.parts * sizeof(ra::Cut));
+    size_t n = round256(rows * c.hd * sizeof(float)) + round256(rows * sizeof(float2)) +
+               round256(pl.parts * sizeof(ra::Cut));
+    if (pl.tc && c.bits != 16) n += group_of(c, a, pl) * (rows_tc_expand_bytes(c, a) + 1024);
+    return n;
 }
 
-cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspace, bool overlap,
+cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& all, void* workspace, bool overlap,
                              cudaStream_t st) {
-    const Plan pl = plan_of(c, a);
+    const Plan pl = plan_of(c, all);
     const size_t rows = 2 * static_cast<size_t>(pl.parts) * pl.rows;
     ra::Params p;
-    p.a = a;
+    p.a = all;
     p.c = c;
-    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.scale_log2 = all.scale * 1.4426950408889634f;
     p.parts = pl.parts;
     char* ws = static_cast<char*>(workspace);
     p.part_o = reinterpret_cast<float*>(ws);
@@ -450,31 +472,46 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspac
     p.part_ml = reinterpret_cast<float2*>(ws);
     ws += round256(rows * sizeof(float2));
     p.cut = reinterpret_cast<ra::Cut*>(ws);
-    void* args[] = {&p};
+    ws += round256(pl.parts * sizeof(ra::Cut));
     const bool bf = c.dtype == kBF16, big = c.hd == 128;
-    const int variant = ((bf ? 0 : 1) * 2 + (big ? 0 : 1)) * 3 + (c.bits == 16 ? 0 : c.bits == 8 ? 1 : 2);
+    const int type = (bf ? 0 : 1) * 2 + (big ? 0 : 1);
     const int size = pl.rows == 8 ? 0 : pl.rows == 16 ? 1 : 2;
-    static PerDevice cfg[36];
-    cudaError_t e;
-    if (pl.tc) {
-        e = launch_ex(rows_tc_fn(c.dtype, c.hd, c.bits), cfg[variant * 3 + size], dim3(pl.parts),
-                      dim3(kRowsTcThreads), rows_tc_smem(c.hd), st, overlap, args);
-    } else {
-        const void* f = bf ? (big ? rows_fn<__nv_bfloat16, 128>(c.bits, pl.rows)
-                                  : rows_fn<__nv_bfloat16, 64>(c.bits, pl.rows))
-                           : (big ? rows_fn<__half, 128>(c.bits, pl.rows)
-                                  : rows_fn<__half, 64>(c.bits, pl.rows));
-        e = launch_ex(f, cfg[variant * 3 + size], dim3(pl.parts), dim3(ra::THREADS), 0, st, overlap,
-                      args);
+    // sequences [b, b + n) at a time; the whole batch but for large expansions
+    const int group = group_of(c, all, pl);
+    for (int b = 0; b < all.batch; b += group) {
+        const int n = all.batch - b < group ? all.batch - b : group;
+        if (group < all.batch) {
+            p.a.cu_q = all.cu_q + b;  // (tcgen05 calls have offsets: a row each is no such call)
+            p.a.kv_lens = all.kv_lens + b;
+            p.a.table = all.table + static_cast<size_t>(b) * all.max_blocks;
+            p.a.batch = n;
+            p.a.tail = all.tail && b + n == all.batch;
+        }
+        void* args[] = {&p};
+        cudaError_t e;
+        if (pl.tc) {
+            e = launch_rows_tc(p, ws, overlap, st);
+        } else {
+            const void* f = bf ? (big ? rows_fn<__nv_bfloat16, 128>(c.bits, pl.rows)
+                                      : rows_fn<__nv_bfloat16, 64>(c.bits, pl.rows))
+                               : (big ? rows_fn<__half, 128>(c.bits, pl.rows)
+                                      : rows_fn<__half, 64>(c.bits, pl.rows));
+            static PerDevice cfg[24];
+            e = launch_ex(f, cfg[(type * 3 + (c.bits == 16 ? 0 : c.bits == 8 ? 1 : 2)) * 2 + size],
+                          dim3(pl.parts), dim3(ra::THREADS), 0, st, overlap, args);
+        }
+        if (e != cudaSuccess) return e;
+        overlap = true;  // (from here on every launch waits for the one before)
+        if (pl.parts == 1) continue;
+        const void* fc = bf ? (big ? combine_fn<__nv_bfloat16, 128>(pl.rows)
+                                   : combine_fn<__nv_bfloat16, 64>(pl.rows))
+                            : (big ? combine_fn<__half, 128>(pl.rows) : combine_fn<__half, 64>(pl.rows));
+        static PerDevice cfgc[12];
+        e = launch_ex(fc, cfgc[type * 3 + size], dim3(pl.parts - 1, (pl.rows + 31) / 32), dim3(256), 0,
+                      st, true, args);
+        if (e != cudaSuccess) return e;
     }
-    if (e != cudaSuccess || pl.parts == 1) return e;
-    const void* fc = bf ? (big ? combine_fn<__nv_bfloat16, 128>(pl.rows)
-                               : combine_fn<__nv_bfloat16, 64>(pl.rows))
-                        : (big ? combine_fn<__half, 128>(pl.rows) : combine_fn<__half, 64>(pl.rows));
-    static PerDevice cfgc[12];
-    // (its launch may begin while the parts are computed; it waits for them all)
-    return launch_ex(fc, cfgc[(variant / 3) * 3 + size], dim3(pl.parts - 1, (pl.rows + 31) / 32),
-                     dim3(256), 0, st, true, args);
+    return cudaSuccess;
 }
 
 }  // namespace mlxq

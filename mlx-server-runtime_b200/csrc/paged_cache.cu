@@ -262,33 +262,7 @@ __global__ void __launch_bounds__(256)
     const int slot = slots[i / cpr];
     uint4 o = make_uint4(0u, 0u, 0u, 0u);
     if (slot >= 0 && slot < c.pages * static_cast<long long>(c.page)) {
-        const size_t at = static_cast<size_t>(slot) * cpr + ch;  // chunk in the pool
-        const void* data = is_v ? c.v : c.k;
-        if constexpr (BITS == 16) {
-            o = static_cast<const uint4*>(data)[at];
-        } else {
-            uint32_t w[BITS / 4];
-            if constexpr (BITS == 8) {
-                const uint2 p = static_cast<const uint2*>(data)[at];
-                w[0] = p.x;
-                w[1] = p.y;
-            } else {
-                w[0] = static_cast<const uint32_t*>(data)[at];
-            }
-            const size_t g = at * 8 / c.gs;
-            const uint32_t s = pk_splat(static_cast<const uint16_t*>(is_v ? c.vs : c.ks)[g]);
-            const uint32_t b = pk_splat(static_cast<const uint16_t*>(is_v ? c.vb : c.kb)[g]);
-            uint32_t p[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = row_pair<T, BITS>(w, j, s, b);
-            if constexpr (BITS == 8) {  // pairs (0,2) (1,3) (4,6) (5,7)
-                o = make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[0], p[1], 0x7632u),
-                               prmt(p[2], p[3], 0x5410u), prmt(p[2], p[3], 0x7632u));
-            } else {  // pairs (0,4) (1,5) (2,6) (3,7)
-                o = make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u),
-                               prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
-            }
-        }
+        o = cache_chunk<T, BITS>(c, is_v, static_cast<size_t>(slot) * cpr + ch);
     }
     reinterpret_cast<uint4*>(is_v ? v_out : k_out)[i] = o;
 }

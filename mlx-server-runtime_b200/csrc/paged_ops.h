@@ -43,17 +43,24 @@ struct RowsArgs {
     const long long* mask;
     int max_blocks, max_kv, max_q, total, batch, Hq;
     float scale;
+    bool tail;  // zero the rows behind the last sequence
 };
-// Bytes of workspace the launch needs (a function of sizes alone; no zero-fill needed).
+// Bytes of workspace the launch needs (a function of sizes alone; no zero-fill needed), and
+// whether its units of work can be counted in 31 bits.
+bool attn_rows_countable(const KvCache& c, const RowsArgs& a);
 size_t attn_rows_workspace(const KvCache& c, const RowsArgs& a);
 cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspace, bool overlap,
                              cudaStream_t st);
 
-// The tcgen05 form of the attention kernel (paged_attn_tc.cu): 128 query rows and kRowsTcKeys
-// keys to a tile.
-constexpr int kRowsTcKeys = 128, kRowsTcThreads = 256;
-const void* rows_tc_fn(int dtype, int hd, int bits);
-size_t rows_tc_smem(int hd);
+// The tcgen05 form of the attention (paged_attn_tc.cu): 128 query rows and kRowsTcKeys keys
+// to a tile, over 16-bit rows; a quantised cache's are expanded into `expanded` first, which
+// takes rows_tc_expand_bytes for each sequence.
+constexpr int kRowsTcKeys = 64, kRowsTcThreads = 256;
+namespace ra {
+struct Params;
+}
+size_t rows_tc_expand_bytes(const KvCache& c, const RowsArgs& a);
+cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStream_t st);
 cudaError_t rows_tc_read_error(int* code);
 
 }  // namespace mlxq

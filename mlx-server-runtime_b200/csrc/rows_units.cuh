@@ -50,28 +50,28 @@ __device__ __forceinline__ Seq seq_of(const RowsArgs& a, int b, int G, int rows)
 }
 
 // Prefix sums of the batch's units, thread i < SCAN over a run of sequences. Every thread of
-// the CTA calls it.
+// the CTA calls it. (The host refuses a call of 2^31 units or more.)
 constexpr int SCAN = 128;
 struct Units {
-    long long total;
+    int total;
     int per;  // sequences per scanning thread
 };
 template <int KT>
 __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, int rows,
-                                            long long* pref /* shared [SCAN + 1] */) {
-    __shared__ long long wsum[SCAN / 32];
+                                            int* pref /* shared [SCAN + 1] */) {
+    __shared__ int wsum[SCAN / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     Units u;
     u.per = (a.batch + SCAN - 1) / SCAN;
-    long long inc = 0;
+    int inc = 0;
     if (tid < SCAN) {
         for (int b = tid * u.per; b < min(a.batch, (tid + 1) * u.per); ++b) {
             const Seq s = seq_of<KT>(a, b, G, rows);
-            inc += static_cast<long long>(s.chunks) * s.tiles * Hkv;
+            inc += s.chunks * s.tiles * Hkv;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= o) inc += v;
         }
         if (lane == 31) wsum[warp] = inc;
@@ -87,26 +87,27 @@ __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, i
     return u;
 }
 
-// A CTA's run of units as segments, each a range of tiles of one item.
+// A CTA's run of units as segments, each a range of tiles of one item. The first `extra`
+// CTAs take share + 1 units, the others share.
 template <int KT, int ROWS>
 struct Walk {
-    long long u, u_lo, u_hi, start, total;
-    int b, G, Hkv, P;
+    int u, u_lo, u_hi, start;
+    int b, G, Hkv, share, extra;
     // the segment
     Seq s;
     int g, rr0, t0, t1;
-    long long item_u0;
 
     __device__ __forceinline__ void begin(const RowsArgs& a, int Hkv_, const Units& un, int parts,
-                                          const long long* pref) {
+                                          const int* pref) {
         Hkv = Hkv_;
         G = a.Hq / Hkv;
-        total = un.total;
-        P = static_cast<int>(min(static_cast<long long>(parts), total));  // no share is empty
-        u = u_lo = u_hi = 0;
-        if (static_cast<int>(blockIdx.x) >= P) return;
-        u = u_lo = total * blockIdx.x / P;
-        u_hi = total * (blockIdx.x + 1) / P;
+        const int P = max(1, min(parts, un.total)), i = blockIdx.x;  // no share is empty
+        share = un.total / P;
+        extra = un.total - share * P;
+        u = u_lo = u_hi = start = b = 0;
+        if (i >= P || un.total == 0) return;
+        u = u_lo = i * share + min(i, extra);
+        u_hi = u + share + (i < extra ? 1 : 0);
         int lo = 0, hi = SCAN - 1;  // the last run of sequences that begins at or before u
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -120,7 +121,7 @@ struct Walk {
     __device__ __forceinline__ bool next(const RowsArgs& a) {
         while (u < u_hi) {
             s = seq_of<KT>(a, b, G, ROWS);
-            const long long n = static_cast<long long>(s.chunks) * s.tiles * Hkv;
+            const int n = s.chunks * s.tiles * Hkv;
             if (u >= start + n) {
                 start += n;
                 ++b;
@@ -128,10 +129,9 @@ struct Walk {
             }
             // kv head fastest outside the tiles: neighbouring runs read neighbouring parts
             // of the same pages
-            const int item = static_cast<int>((u - start) / s.tiles);
-            t0 = static_cast<int>((u - start) % s.tiles);
-            t1 = static_cast<int>(min(static_cast<long long>(s.tiles), t0 + (u_hi - u)));
-            item_u0 = u - t0;
+            const int item = (u - start) / s.tiles;
+            t0 = (u - start) - item * s.tiles;
+            t1 = min(s.tiles, t0 + (u_hi - u));
             g = item % Hkv;
             rr0 = item / Hkv * ROWS;
             return true;
@@ -148,15 +148,20 @@ struct Walk {
         const int last = min(s.n * G, rr0 + ROWS) - 1;
         return max(0, a.mask ? s.L : min(s.L, base() + last / G + 1));
     }
-    // The CTA that owns unit x of the run of all.
-    __device__ __forceinline__ int owner(long long x) const {
-        return static_cast<int>(((x + 1) * P - 1) / total);
+    // tiles of the segment that hold such keys
+    __device__ __forceinline__ int tile_end(const RowsArgs& a) const {
+        return min(t1, (kend(a) + KT - 1) / KT);
+    }
+    // The CTA that owns unit x.
+    __device__ __forceinline__ int owner(int x) const {
+        const int big = extra * (share + 1);
+        return x < big ? x / (share + 1) : extra + (x - big) / share;
     }
     __device__ __forceinline__ Cut cut() const {
         Cut c;
         c.rows = min(s.n * G - rr0, ROWS);
         c.slot = slot();
-        c.last = owner(item_u0 + s.tiles - 1);
+        c.last = owner(u - t0 + s.tiles - 1);
         c.row0 = s.row0;
         c.rr0 = rr0;
         c.g = g;
@@ -166,7 +171,7 @@ struct Walk {
 
 // Rows behind the last sequence are zero.
 __device__ __forceinline__ void zero_tail(const RowsArgs& a, int HD, int threads) {
-    if (!a.cu_q) return;
+    if (!a.cu_q || !a.tail) return;
     const long long row = static_cast<long long>(a.Hq) * HD / 8;
     const int end = max(0, min(a.cu_q[a.batch], a.total));
     uint4* o = static_cast<uint4*>(a.out);

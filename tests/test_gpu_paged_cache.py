@@ -365,12 +365,32 @@ def test_lengths_past_their_bounds_stay_in_bounds():
     torch.cuda.synchronize()
 
 
-def test_large_scores_and_equal_keys():
+@pytest.mark.parametrize("how,bits", [("decode", 8), ("tree", 4), ("tree", 16), ("prefill", 8)])
+def test_large_scores_and_equal_keys(how, bits):
     """Scores far apart (one key takes all), equal scores, and a scale of zero."""
-    p = _problem(10, HF, 8, 64, 8, 2, 64, 16, [200, 77, 64], [1] * 3)
+    news = [1] * 3 if how == "decode" else [50, 3, 64]
+    p = _problem(10, HF, bits, 64, 8, 2, 64, 16, [200, 77, 64], news, tree=how == "tree")
     for scale in (0.0, 4.0, -0.3):
         p["scale"] = scale
-        _check(p, _run(p, "decode"))
+        _check(p, _run(p, how))
+
+
+def test_rising_scores():
+    """The largest score grows tile after tile, so what is summed so far is rescaled again
+    and again."""
+    for how, bits in (("decode", 8), ("tree", 16), ("prefill", 4)):
+        news = [1] if how == "decode" else [40]
+        p = _problem(12, BF, bits, 64, 8, 2, 64, 16, [1500], news, tree=how == "tree")
+        t = torch.linspace(0, 1, p["table"]["pages"] * 16, device="cuda")
+        order = torch.zeros(p["table"]["pages"] * 16, device="cuda")
+        rows = [p["table"]["rows"][0][j // 16] * 16 + j % 16 for j in range(1500)]
+        order[rows] = t[:1500]
+        k = (p["q"][0, 0].float() * order[:, None, None]).to(BF).expand(-1, 2, -1)
+        k = k.reshape(p["table"]["pages"], 16, 2, 64).contiguous()
+        p["kc"] = k if bits == 16 else quantized_pool(k, 64, bits)
+        p["kd"] = pool_values(p["kc"])
+        p["scale"] = 8.0
+        _check(p, _run(p, how))
 
 
 def test_same_result_every_time():
