@@ -336,52 +336,61 @@ __global__ void __launch_bounds__(ra::THREADS)
     if (tid == 0) p.cut[blockIdx.x] = mine;
 }
 
-// Joins the parts of the items that several CTAs took: block (CTA that began one, group of
-// 32 rows), warp = row, lane = HD / 32 dimensions. Parts are taken in order of keys.
+// Joins the parts of the items that several CTAs took: block (CTA that began one, eight
+// rows), warp = row, lane = HD / 32 dimensions. Parts are taken in order of keys, eight
+// loads ahead.
 template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant__ ra::Params p) {
     using namespace ra;
-    constexpr int DPL = HD / 32;
+    constexpr int DPL = HD / 32, AHEAD = 8;
     pdl_launch_dependents();
     pdl_wait();
     const Cut c = p.cut[blockIdx.x];
     const RowsArgs& a = p.a;
     const int G = a.Hq / p.c.Hkv, lane = threadIdx.x & 31;
-    const int end = min(c.rows, static_cast<int>(blockIdx.y + 1) * 32);
-    for (int r = blockIdx.y * 32 + (threadIdx.x >> 5); r < end; r += 8) {
-        float M = -INFINITY, den = 0.f, acc[DPL];
+    const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (r >= c.rows) return;
+    const int first = blockIdx.x;
+    float M = -INFINITY, den = 0.f, acc[DPL];
 #pragma unroll
-        for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
-#pragma unroll 4
-        for (int k = blockIdx.x; k <= c.last; ++k) {
-            const size_t at = static_cast<size_t>(k == blockIdx.x ? c.slot : 2 * k) * ROWS + r;
-            const float2 ml = __ldcg(&p.part_ml[at]);
-            float v[DPL];
+    for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
+    for (int k0 = first; k0 <= c.last; k0 += AHEAD) {
+        float2 ml[AHEAD];
+        float v[AHEAD][DPL];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int k = min(k0 + i, c.last);
+            const size_t at = static_cast<size_t>(k == first ? c.slot : 2 * k) * ROWS + r;
+            ml[i] = __ldcg(&p.part_ml[at]);
             if constexpr (DPL == 4) {
                 const float4 t = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * HD) + lane);
-                v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+                v[i][0] = t.x; v[i][1] = t.y; v[i][2] = t.z; v[i][3] = t.w;
             } else {
                 const float2 t = __ldcg(reinterpret_cast<const float2*>(p.part_o + at * HD) + lane);
-                v[0] = t.x; v[1] = t.y;
+                v[i][0] = t.x; v[i][1] = t.y;
             }
-            const float Mn = fmaxf(M, ml.x);
-            const float co = M == -INFINITY ? 0.f : exp2f(M - Mn);
-            const float cn = ml.x == -INFINITY ? 0.f : exp2f(ml.x - Mn);
-            den = fmaf(cn, ml.y, den * co);
+        }
 #pragma unroll
-            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(cn, v[e], acc[e] * co);
+        for (int i = 0; i < AHEAD; ++i) {
+            if (k0 + i > c.last) break;
+            const float Mn = fmaxf(M, ml[i].x);
+            const float co = M == -INFINITY ? 0.f : exp2f(M - Mn);
+            const float cn = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - Mn);
+            den = fmaf(cn, ml[i].y, den * co);
+#pragma unroll
+            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(cn, v[i][e], acc[e] * co);
             M = Mn;
         }
-        const float inv = M == -INFINITY ? 0.f : 1.0f / den;
-        const int rr = c.rr0 + r;
-        T* dst = static_cast<T*>(a.out) +
-                 (static_cast<size_t>(c.row0 + rr / G) * a.Hq + c.g * G + rr % G) * HD + lane * DPL;
-        if constexpr (DPL == 4)
-            *reinterpret_cast<uint2*>(dst) = make_uint2(pk_round<T>(acc[0] * inv, acc[1] * inv),
-                                                        pk_round<T>(acc[2] * inv, acc[3] * inv));
-        else
-            *reinterpret_cast<uint32_t*>(dst) = pk_round<T>(acc[0] * inv, acc[1] * inv);
     }
+    const float inv = M == -INFINITY ? 0.f : 1.0f / den;
+    const int rr = c.rr0 + r;
+    T* dst = static_cast<T*>(a.out) +
+             (static_cast<size_t>(c.row0 + rr / G) * a.Hq + c.g * G + rr % G) * HD + lane * DPL;
+    if constexpr (DPL == 4)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pk_round<T>(acc[0] * inv, acc[1] * inv),
+                                                    pk_round<T>(acc[2] * inv, acc[3] * inv));
+    else
+        *reinterpret_cast<uint32_t*>(dst) = pk_round<T>(acc[0] * inv, acc[1] * inv);
 }
 
 namespace {
@@ -507,7 +516,7 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& all, void* worksp
                                    : combine_fn<__nv_bfloat16, 64>(pl.rows))
                             : (big ? combine_fn<__half, 128>(pl.rows) : combine_fn<__half, 64>(pl.rows));
         static PerDevice cfgc[12];
-        e = launch_ex(fc, cfgc[type * 3 + size], dim3(pl.parts - 1, (pl.rows + 31) / 32), dim3(256), 0,
+        e = launch_ex(fc, cfgc[type * 3 + size], dim3(pl.parts - 1, pl.rows / 8), dim3(256), 0,
                       st, true, args);
         if (e != cudaSuccess) return e;
     }

@@ -152,8 +152,9 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     // phase j >> 1; item i the queries' barriers' phase i. No role is ever two phases behind
     // another: each buffer's next use waits for its last.
     auto wait_at = [&](uint64_t* bar, uint32_t parity) -> bool {
-        if (s_abort) return false;
-        if (mbar_wait_park(smem_u32(bar), parity & 1, kParkLimit, kParkNs)) return true;
+        if (mbar_try_wait(smem_u32(bar), parity & 1)) return true;
+        for (uint32_t i = 0; i < kParkLimit && !s_abort; ++i)
+            if (mbar_try_wait_hint(smem_u32(bar), parity & 1, kParkNs)) return true;
         atomicCAS(&g_rows_tc_error, 0, kErrTimeout);
         s_abort = 1;
         return false;
@@ -273,59 +274,64 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         }
     } else if (warp == WARP_MMA) {
         // ------------------------------ products -------------------------------------
-        if (lane == 0) {
-            auto spin = [&](uint64_t* bar, uint32_t parity) -> bool {
-                // (polls without parking: it wakes fastest)
-                if (!s_abort && mbar_wait_bounded(smem_u32(bar), parity & 1, kSpinLimit)) return true;
-                atomicCAS(&g_rows_tc_error, 0, kErrTimeout);
-                s_abort = 1;
-                return false;
-            };
-            const uint64_t qd = sw128_kmajor_desc(smem_u32(qs)), kd = sw128_kmajor_desc(smem_u32(ks));
-            const uint64_t vd = sw128_mnmajor_desc(smem_u32(vs), KT * 128);
-            uint32_t ns = 0, npv = 0, nq = 0;  // S and P V issued, items of queries met
-            uint32_t begins = 0;               // tiles that begin an item, by their last five bits
-            bool ok = true, more = true;
-            auto issue_s = [&]() {             // of the next tile, if there is one
-                if (!(more = step())) return;
-                const bool begin = tile == w.t0;
-                const uint32_t bit = 1u << (ns & 31);
-                begins = begin ? begins | bit : begins & ~bit;
-                if ((begin && !spin(&q_full, nq++)) || !spin(k_full + (ns & 1), ns >> 1)) {
-                    ok = false;
-                    return;
-                }
-                tc_fence_after();
-                const uint64_t kb = kd + (ns & 1) * (HB / 16);
-                const uint32_t d = tmem + (ns & 1) * KT;
-#pragma unroll
-                for (int i = 0; i < HD / 16; ++i)  // 16 dims: 32 bytes of a half of them
-                    umma_f16_ss(d, qd + (i / 4) * (ROWS * 128 / 16) + (i % 4) * 2,
-                                kb + (i / 4) * (KT * 128 / 16) + (i % 4) * 2, IDESC_S, i > 0 ? 1u : 0u);
-                umma_commit(smem_u32(s_full + (ns & 1)));
-                if (tile + 1 == te) umma_commit(smem_u32(&q_free));
-                ++ns;
-            };
-            issue_s();
-            if (ok && more) issue_s();
-            while (ok && npv < ns) {
-                if (!spin(v_full + (npv & 1), npv >> 1) || !spin(p_full + (npv & 1), npv >> 1)) break;
-                tc_fence_after();
-                const uint64_t vb = vd + (npv & 1) * (HB / 16);
-                const uint32_t pa = tmem + (npv & 1) * KT;
-                const bool begin = begins >> (npv & 31) & 1;
-#pragma unroll
-                for (int i = 0; i < KT / 16; ++i)  // 16 keys: 8 columns of P, 2 KB of V
-                    umma_f16_ts(tmem + kOCol, pa + 8 * i, vb + i * (2048 / 16), IDESC_O,
-                                (!begin || i > 0) ? 1u : 0u);
-                umma_commit(smem_u32(pv_done + (npv & 1)));
-                ++npv;
-                if (more) issue_s();
+        // The whole warp walks along, so that descriptors stay in uniform registers (by one
+        // thread in a branch of its own, issuing took 2600 cycles a tile, twice what the
+        // softmax takes); one thread of it issues.
+        const uint32_t leader = elect_leader();
+        auto spin = [&](uint64_t* bar, uint32_t parity) -> bool {
+            // (polls without parking: it wakes fastest)
+            if (mbar_wait_bounded(smem_u32(bar), parity & 1, 64)) return true;
+            for (uint32_t i = 0; i < kSpinLimit / 64 && !s_abort; ++i)
+                if (mbar_wait_bounded(smem_u32(bar), parity & 1, 64)) return true;
+            atomicCAS(&g_rows_tc_error, 0, kErrTimeout);
+            s_abort = 1;
+            return false;
+        };
+        const uint64_t qd = sw128_kmajor_desc(smem_u32(qs)), kd = sw128_kmajor_desc(smem_u32(ks));
+        const uint64_t vd = sw128_mnmajor_desc(smem_u32(vs), KT * 128);
+        uint32_t ns = 0, npv = 0, nq = 0;  // S and P V issued, items of queries met
+        uint32_t begins = 0;               // tiles that begin an item, by their last five bits
+        bool ok = true, more = true;
+        auto issue_s = [&]() {             // of the next tile, if there is one
+            if (!(more = step())) return;
+            const bool begin = tile == w.t0;
+            const uint32_t bit = 1u << (ns & 31), buf = ns & 1;
+            begins = begin ? begins | bit : begins & ~bit;
+            if ((begin && !spin(&q_full, nq++)) || !spin(k_full + buf, ns >> 1)) {
+                ok = false;
+                return;
             }
-            // every product issued has finished before tensor memory is freed
-            umma_commit(smem_u32(&drained));
-            mbar_wait_bounded(smem_u32(&drained), 0, kSpinLimit);
+            tc_fence_after();
+            const uint64_t kb = kd + buf * (HB / 16);
+            const uint32_t d = tmem + buf * KT;
+#pragma unroll
+            for (int i = 0; i < HD / 16; ++i)  // 16 dims: 32 bytes of a half of them
+                umma_f16_ss_by(leader, d, qd + (i / 4) * (ROWS * 128 / 16) + (i % 4) * 2,
+                               kb + (i / 4) * (KT * 128 / 16) + (i % 4) * 2, IDESC_S, i > 0 ? 1u : 0u);
+            umma_commit_by(leader, smem_u32(s_full + buf));
+            if (tile + 1 == te) umma_commit_by(leader, smem_u32(&q_free));
+            ++ns;
+        };
+        issue_s();
+        if (ok && more) issue_s();
+        while (ok && npv < ns) {
+            const uint32_t buf = npv & 1;
+            if (!spin(v_full + buf, npv >> 1) || !spin(p_full + buf, npv >> 1)) break;
+            tc_fence_after();
+            const uint64_t vb = vd + buf * (HB / 16);
+            const uint32_t pa = tmem + buf * KT;
+            const bool begin = begins >> (npv & 31) & 1;
+#pragma unroll
+            for (int i = 0; i < KT / 16; ++i)  // 16 keys: 8 columns of P, 2 KB of V
+                umma_f16_ts_by(leader, tmem + kOCol, pa + 8 * i, vb + i * (2048 / 16), IDESC_O,
+                               (!begin || i > 0) ? 1u : 0u);
+            umma_commit_by(leader, smem_u32(pv_done + buf));
+            ++npv;
+            if (more) issue_s();
         }
+        // every product issued has finished before tensor memory is freed
+        umma_commit_by(leader, smem_u32(&drained));
+        mbar_wait_bounded(smem_u32(&drained), 0, kSpinLimit);
     } else {
         // ------------------------------ softmax, epilogue -----------------------------
         const int row = tid;  // of the tile; tensor-memory lane
@@ -490,30 +496,30 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
 }
 
 // The values of every sequence's keys, from the first to the end of its last tile (zeros
-// behind the last key and for pages outside the pool): thread = eight dims of a head of key
-// blockIdx.x * 256 / (chunks of a row) .. of sequence blockIdx.y; keys' (blockIdx.z 0) or
-// values' pool.
+// behind the last key and for pages outside the pool): block (eight keys, sequence, keys or
+// values), thread = eight dims of a head at a time. Eight keys share a page.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
     kv_expand_kernel(const KvCache c, const RowsArgs a, int rows_per_seq, T* __restrict__ k_out,
                      T* __restrict__ v_out) {
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.y, cpr = c.Hkv * c.hd / 8;
+    const int b = blockIdx.y, cpr = c.Hkv * c.hd / 8, key = blockIdx.x * 8;
     const int L = max(0, min(a.kv_lens[b], a.max_kv));
-    const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int key = static_cast<int>(i / cpr), ch = static_cast<int>(i - static_cast<long long>(key) * cpr);
     if (key >= (L + rt::KT - 1) / rt::KT * rt::KT) return;
-    uint4 o = make_uint4(0u, 0u, 0u, 0u);
-    if (key < L) {
-        const int pid = __ldg(a.table + static_cast<size_t>(b) * a.max_blocks + key / c.page);
-        if (pid >= 0 && pid < c.pages) {
-            const size_t at = (static_cast<size_t>(pid) * c.page + key % c.page) * cpr + ch;
-            o = cache_chunk<T, BITS>(c, blockIdx.z != 0, at);
-        }
+    int pid = -1;
+    if (key < L) pid = __ldg(a.table + static_cast<size_t>(b) * a.max_blocks + key / c.page);
+    const bool there = pid >= 0 && pid < c.pages;
+    const size_t from = there ? (static_cast<size_t>(pid) * c.page + key % c.page) * cpr : 0;
+    uint4* out = reinterpret_cast<uint4*>(blockIdx.z ? v_out : k_out) +
+                 (static_cast<size_t>(b) * rows_per_seq + key) * cpr;
+    const int n = there ? min(8, L - key) * cpr : 0;  // chunks that hold values
+#pragma unroll 4
+    for (int i = threadIdx.x; i < 8 * cpr; i += 256) {
+        uint4 o = make_uint4(0u, 0u, 0u, 0u);
+        if (i < n) o = cache_chunk<T, BITS>(c, blockIdx.z != 0, from + i);
+        out[i] = o;
     }
-    reinterpret_cast<uint4*>(blockIdx.z ? v_out : k_out)
-        [(static_cast<size_t>(b) * rows_per_seq + key) * cpr + ch] = o;
 }
 
 namespace {
@@ -570,7 +576,6 @@ cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStre
         if (rps == 0) rps = rt::KT;
         const size_t each = static_cast<size_t>(p.a.batch) * rps * c.Hkv * c.hd * 2;
         void *ko = expanded, *vo = static_cast<char*>(expanded) + each;
-        const unsigned blocks = static_cast<unsigned>((static_cast<long long>(rps) * (c.Hkv * c.hd / 8) + 255) / 256);
         KvCache cc = c;
         RowsArgs aa = p.a;
         void* args[] = {&cc, &aa, &rps, &ko, &vo};
@@ -580,7 +585,7 @@ cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStre
                                           : reinterpret_cast<const void*>(&kv_expand_kernel<__half, 4>));
         static PerDevice cfg[4];
         const cudaError_t e = launch_ex(f, cfg[(bf ? 0 : 2) + (c.bits == 8 ? 0 : 1)],
-                                        dim3(blocks, p.a.batch, 2), dim3(256), 0, st, overlap, args);
+                                        dim3(rps / 8, p.a.batch, 2), dim3(256), 0, st, overlap, args);
         if (e != cudaSuccess) return e;
         overlap = true;  // (the attention waits for the whole of it)
         k = ko;
