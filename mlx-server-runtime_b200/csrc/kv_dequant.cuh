@@ -43,6 +43,12 @@ __device__ __forceinline__ uint32_t pk_round(float a, float b) {  // a in the lo
         return *reinterpret_cast<const uint32_t*>(&r);
     }
 }
+__device__ __forceinline__ float ex2(float x) {  // 2^x, results below 2^-126 as zero
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // Two 4-bit codes at bits 0-3 and 16-19 of h (other bits arbitrary) as an exact pair.
 template <typename T>
 __device__ __forceinline__ uint32_t nibbles_pair(uint32_t h) {
@@ -103,6 +109,20 @@ __device__ __forceinline__ uint32_t cross_pair(const uint32_t* wa, const uint32_
     }
 }
 
+// Eight values in order from the words that hold them.
+template <typename T, int BITS>
+__device__ __forceinline__ uint4 in_order(const uint32_t* w, uint32_t s2, uint32_t b2) {
+    uint32_t p[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = row_pair<T, BITS>(w, j, s2, b2);
+    if constexpr (BITS == 8)  // pairs (0,2) (1,3) (4,6) (5,7)
+        return make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[0], p[1], 0x7632u),
+                          prmt(p[2], p[3], 0x5410u), prmt(p[2], p[3], 0x7632u));
+    // pairs (0,4) (1,5) (2,6) (3,7)
+    return make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u),
+                      prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
+}
+
 // Eight values of a pool: chunk `at` of eight elements of its rows.
 template <typename T, int BITS>
 __device__ __forceinline__ uint4 cache_chunk(const KvCache& c, bool is_v, size_t at) {
@@ -110,7 +130,7 @@ __device__ __forceinline__ uint4 cache_chunk(const KvCache& c, bool is_v, size_t
     if constexpr (BITS == 16) {
         return static_cast<const uint4*>(data)[at];
     } else {
-        uint32_t w[BITS / 4], p[4];
+        uint32_t w[BITS / 4];
         if constexpr (BITS == 8) {
             const uint2 v = static_cast<const uint2*>(data)[at];
             w[0] = v.x;
@@ -119,16 +139,8 @@ __device__ __forceinline__ uint4 cache_chunk(const KvCache& c, bool is_v, size_t
             w[0] = static_cast<const uint32_t*>(data)[at];
         }
         const size_t g = at * 8 / c.gs;
-        const uint32_t s = pk_splat(static_cast<const uint16_t*>(is_v ? c.vs : c.ks)[g]);
-        const uint32_t b = pk_splat(static_cast<const uint16_t*>(is_v ? c.vb : c.kb)[g]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = row_pair<T, BITS>(w, j, s, b);
-        if constexpr (BITS == 8)  // pairs (0,2) (1,3) (4,6) (5,7)
-            return make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[0], p[1], 0x7632u),
-                              prmt(p[2], p[3], 0x5410u), prmt(p[2], p[3], 0x7632u));
-        // pairs (0,4) (1,5) (2,6) (3,7)
-        return make_uint4(prmt(p[0], p[1], 0x5410u), prmt(p[2], p[3], 0x5410u),
-                          prmt(p[0], p[1], 0x7632u), prmt(p[2], p[3], 0x7632u));
+        return in_order<T, BITS>(w, pk_splat(static_cast<const uint16_t*>(is_v ? c.vs : c.ks)[g]),
+                                 pk_splat(static_cast<const uint16_t*>(is_v ? c.vb : c.kb)[g]));
     }
 }
 

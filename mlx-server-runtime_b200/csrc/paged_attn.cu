@@ -41,17 +41,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
 }
 
 template <int N>
-__device__ __forceinline__ void ldw(const uint32_t* p, uint32_t (&r)[N]) {
+__device__ __forceinline__ void ldw(const void* at, uint32_t (&r)[N]) {
     if constexpr (N == 1) {
-        r[0] = *p;
+        r[0] = __ldg(static_cast<const uint32_t*>(at));
     } else if constexpr (N == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        const uint2 v = __ldg(static_cast<const uint2*>(at));
         r[0] = v.x;
         r[1] = v.y;
     } else {
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
-            const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+            const uint4 v = __ldg(static_cast<const uint4*>(at) + i);
             r[4 * i] = v.x;
             r[4 * i + 1] = v.y;
             r[4 * i + 2] = v.z;
@@ -59,16 +59,28 @@ __device__ __forceinline__ void ldw(const uint32_t* p, uint32_t (&r)[N]) {
         }
     }
 }
+
+// CTAs of an SM: what the registers of a variant allow (and the launch bounds ask for).
+constexpr int resident(int hd, int bits, int nt) {
+    return nt == 2 ? 2 : hd == 64 ? 4 : bits == 4 ? 4 : bits == 8 ? 3 : 2;
+}
+
+// A lane's part of 16 keys on its way: words of key rows r8 and r8 + 8 (a quarter of each),
+// of value rows 2 c4, 2 c4 + 1 and eight on (an eighth of each); and of (key lane % 16,
+// group lane / 16, and with four groups lane / 16 + 2) scale | bias << 16.
+template <int HD, int BITS>
+struct Raw {
+    uint32_t k[2][HD / 4 * BITS / 32], v[4][HD / 8 * BITS / 32];
+    uint32_t ks[2], vs[2];
+};
 }  // namespace ra
 
 template <typename T, int HD, int BITS, int NT>
-__global__ void __launch_bounds__(ra::THREADS)
+__global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
     attn_rows_kernel(const __grid_constant__ ra::Params p) {
     using namespace ra;
     constexpr int ROWS = 8 * NT;
-    constexpr int KW = HD / 4 * BITS / 32;  // words of a key row per lane (a quarter)
-    constexpr int VW = HD / 8 * BITS / 32;  // words of a value row per lane (an eighth)
-    constexpr int RW = HD * BITS / 32;      // words of a row
+    constexpr int RB = HD * BITS / 8;  // bytes of a row
     constexpr int MT = HD / 16;
     __shared__ int pref[SCAN + 1];
     __shared__ float wo[WARPS][ROWS][HD + 4];
@@ -79,33 +91,31 @@ __global__ void __launch_bounds__(ra::THREADS)
     const KvCache& c = p.c;
     const int Hkv = c.Hkv, G = a.Hq / Hkv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r8 = lane >> 2, c4 = lane & 3;
+    const int page_shift = 31 - __clz(c.page);
     const T* q = static_cast<const T*>(a.q);
     T* out = static_cast<T*>(a.out);
 
     zero_tail(a, HD, THREADS);
-    const Units un = scan_units<KT>(a, Hkv, G, ROWS, pref);
+    const Units un = scan_units<KT>(a, Hkv, G, ROWS, p.group, pref);
     Walk<KT, ROWS> w;
-    w.begin(a, Hkv, un, p.parts, pref);
+    w.begin(a, Hkv, un, p.parts, p.group, pref);
     Cut mine = {};
 
-    const uint32_t* kd = static_cast<const uint32_t*>(c.k);
-    const uint32_t* vd = static_cast<const uint32_t*>(c.v);
-    const uint16_t *ksd = static_cast<const uint16_t*>(c.ks), *kbd = static_cast<const uint16_t*>(c.kb);
-    const uint16_t *vsd = static_cast<const uint16_t*>(c.vs), *vbd = static_cast<const uint16_t*>(c.vb);
     const int ng = BITS == 16 ? 1 : HD / c.gs;
     const int kg = BITS == 16 ? 0 : c4 * (HD / 4) / c.gs;  // this lane's group of a key row
     const int vg = BITS == 16 ? 0 : r8 * (HD / 8) / c.gs;  // and of a value row
+    const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * RB;  // of a token: its heads' rows
 
     for (; w.next(a); w.advance()) {
         const Seq& s = w.s;
-        const int g = w.g, row_lo = w.rr0, t0 = w.t0, b = w.b, R = s.n * G;
+        const int g = w.g, row_lo = w.rr0, t0 = w.t0, R = s.n * G;
         const int base = w.base(), kend = w.kend(a), full = min(max(base, 0), kend);
-        const int32_t* bt = a.table + static_cast<size_t>(b) * a.max_blocks;
+        const int32_t* bt = a.table + static_cast<size_t>(w.b) * a.max_blocks;
 
         // Queries: lane (row r8 of the n-tile, quarter c4) holds its quarter's dims in the
         // order the key words unpack to.
         uint32_t bq[NT][MT][2];
-        int qpos[NT][2];              // column 2 c4 + e: its index among the new tokens
+        int qpos[NT][2];                // column 2 c4 + e: its index among the new tokens
         unsigned long long vis[NT][2];  // and its ancestors
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -114,9 +124,8 @@ __global__ void __launch_bounds__(ra::THREADS)
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) qw[i] = 0u;
             if (rr < R)
-                ldw(reinterpret_cast<const uint32_t*>(
-                        q + (static_cast<size_t>(s.row0 + rr / G) * a.Hq + g * G + rr % G) * HD +
-                        c4 * (HD / 4)),
+                ldw(q + (static_cast<size_t>(s.row0 + rr / G) * a.Hq + g * G + rr % G) * HD +
+                        c4 * (HD / 4),
                     qw);
 #pragma unroll
             for (int i = 0; i < HD / 8; ++i) {
@@ -132,6 +141,7 @@ __global__ void __launch_bounds__(ra::THREADS)
                 if (a.mask) vis[nt][e] = rc < R ? static_cast<unsigned long long>(a.mask[s.row0 + rc / G]) : 0ull;
             }
         }
+
         float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -141,110 +151,112 @@ __global__ void __launch_bounds__(ra::THREADS)
             l[nt][0] = l[nt][1] = 0.f;
         }
 
-        // One 16-key tile per warp and step; the next tile's words are loaded while this
-        // one is multiplied.
-        uint32_t kw[2][KW], vw[4][VW], ksb[2], vsb[2][2];  // (scale, bias) / pairs of keys
-        bool okk[2];
-        auto load = [&](int tile) {
-            const int k0 = tile * KT + warp * 16;
-            const uint32_t *kr[2], *vr[2];
-            size_t row[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {  // eight keys share a page
-                const int key = k0 + 8 * h;
-                int pid = -1;
-                if (key < kend) pid = bt[key / c.page];
-                okk[h] = pid >= 0 && pid < c.pages;
-                row[h] = okk[h] ? (static_cast<size_t>(pid) * c.page + key % c.page) * Hkv + g
-                                : static_cast<size_t>(g);
-                kr[h] = kd + (row[h] + (okk[h] ? static_cast<size_t>(r8) * Hkv : 0)) * RW + c4 * KW;
-                vr[h] = vd + (row[h] + (okk[h] ? static_cast<size_t>(2 * c4) * Hkv : 0)) * RW + r8 * VW;
-            }
+        // Sixteen keys per warp and step. Eight keys share a page: the two page ids of a
+        // step are loaded a step before its rows, the rows a step before their use (16-bit
+        // rows, which would not fit registers twice, K after S and V after P V).
+        const int te = w.tile_end(a);
+        auto pages = [&](int tile, int (&pid)[2]) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                ldw(kr[h], kw[h]);
-                ldw(vr[h], vw[2 * h]);
-                ldw(vr[h] + (okk[h] ? static_cast<size_t>(Hkv) * RW : 0), vw[2 * h + 1]);
+                const int key = tile * KT + warp * 16 + 8 * h;
+                pid[h] = key < kend ? __ldg(bt + (key >> page_shift)) : -1;
+            }
+        };
+        // rows of the pool the two eights begin at; which of them are there, a bit each
+        auto rows = [&](int tile, const int (&pid)[2], uint32_t (&row)[2]) -> uint32_t {
+            uint32_t ok = 0;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool good = pid[h] >= 0 && pid[h] < c.pages;
+                const uint32_t in = static_cast<uint32_t>(tile * KT + warp * 16 + 8 * h) & (c.page - 1);
+                ok |= good ? 1u << h : 0u;
+                row[h] = good ? (static_cast<uint32_t>(pid[h]) << page_shift) + in : 0u;  // (page 0: in bounds)
+            }
+            return ok;
+        };
+        auto load_k = [&](Raw<HD, BITS>& x, const uint32_t (&row)[2]) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                ldw(static_cast<const char*>(c.k) + static_cast<size_t>(row[h] + r8) * row_bytes + g * RB +
+                        c4 * (RB / 4),
+                    x.k[h]);
+        };
+        auto load_v = [&](Raw<HD, BITS>& x, const uint32_t (&row)[2]) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const char* at = static_cast<const char*>(c.v) +
+                                 static_cast<size_t>(row[h] + 2 * c4) * row_bytes + g * RB + r8 * (RB / 8);
+                ldw(at, x.v[2 * h]);
+                ldw(at + row_bytes, x.v[2 * h + 1]);
             }
             if constexpr (BITS != 16) {
+                const size_t token = row[lane >> 3 & 1] + (lane & 7);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const size_t ki = (row[h] + (okk[h] ? static_cast<size_t>(r8) * Hkv : 0)) * ng + kg;
-                    ksb[h] = ksd[ki] | static_cast<uint32_t>(kbd[ki]) << 16;
-                    const size_t step = okk[h] ? static_cast<size_t>(Hkv) * ng : 0;
-                    const size_t vi = row[h] * ng + vg + 2 * c4 * step;
-                    vsb[h][0] = vsd[vi] | static_cast<uint32_t>(vsd[vi + step]) << 16;
-                    vsb[h][1] = vbd[vi] | static_cast<uint32_t>(vbd[vi + step]) << 16;
+                for (int i = 0; i < 2; ++i) {
+                    if (i == 1 && ng < 4) break;
+                    const size_t at = (token * Hkv + g) * ng + min(lane >> 4, ng - 1) + 2 * i;
+                    x.ks[i] = __ldg(static_cast<const uint16_t*>(c.ks) + at) |
+                              static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(c.kb) + at)) << 16;
+                    x.vs[i] = __ldg(static_cast<const uint16_t*>(c.vs) + at) |
+                              static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(c.vb) + at)) << 16;
                 }
             }
         };
-        const int te = w.tile_end(a);
-        if (t0 < te) load(t0);
-        for (int tile = t0; tile < te; ++tile) {
+        // scale | bias of (key, this lane's group) from the lane that loaded it
+        auto sb_of = [&](const uint32_t (&x)[2], int key, int group) -> uint32_t {
+            const int from = key + 16 * (group & 1);
+            uint32_t r = __shfl_sync(0xffffffffu, x[0], from);
+            if (ng == 4) {
+                const uint32_t hi = __shfl_sync(0xffffffffu, x[1], from);
+                r = group & 2 ? hi : r;
+            }
+            return r;
+        };
+
+        auto tile_of = [&](int tile, Raw<HD, BITS>& x, uint32_t ok, auto after_s, auto after_pv) {
             const int k0 = tile * KT + warp * 16;
-            // values of keys that are not there multiply zeros: make them zeros
-            const bool clean = k0 + 16 <= kend && okk[0] && okk[1];
-            if (!clean) {
+            const bool clean = k0 + 16 <= kend && ok == 3u;
+            float sc[NT][4];
+            {
+                uint32_t s2[2] = {0u, 0u}, b2[2] = {0u, 0u};
+                if constexpr (BITS != 16) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = k0 + 8 * h + 2 * c4;
-                    const uint32_t keep = (okk[h] && k < kend ? 0xffffu : 0u) |
-                                          (okk[h] && k + 1 < kend ? 0xffff0000u : 0u);
-                    if constexpr (BITS == 16) {
-#pragma unroll
-                        for (int i = 0; i < VW; ++i) {
-                            if (!(keep & 0xffffu)) vw[2 * h][i] = 0u;
-                            if (!(keep >> 16)) vw[2 * h + 1][i] = 0u;
-                        }
-                    } else {
-                        vsb[h][0] &= keep;
-                        vsb[h][1] &= keep;
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t sb = sb_of(x.ks, r8 + 8 * h, kg);
+                        s2[h] = pk_splat(sb);
+                        b2[h] = prmt(sb, 0u, 0x3232u);
                     }
                 }
-            }
-            float sc[NT][4];
-            uint32_t va[MT][4];
-            {
-                const uint32_t s0 = pk_splat(ksb[0]), b0 = prmt(ksb[0], 0u, 0x3232u);
-                const uint32_t s1 = pk_splat(ksb[1]), b1 = prmt(ksb[1], 0u, 0x3232u);
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
-                    const uint32_t a0 = row_pair<T, BITS>(kw[0], 2 * j, s0, b0);
-                    const uint32_t a1 = row_pair<T, BITS>(kw[1], 2 * j, s1, b1);
-                    const uint32_t a2 = row_pair<T, BITS>(kw[0], 2 * j + 1, s0, b0);
-                    const uint32_t a3 = row_pair<T, BITS>(kw[1], 2 * j + 1, s1, b1);
+                    const uint32_t a0 = row_pair<T, BITS>(x.k[0], 2 * j, s2[0], b2[0]);
+                    const uint32_t a1 = row_pair<T, BITS>(x.k[1], 2 * j, s2[1], b2[1]);
+                    const uint32_t a2 = row_pair<T, BITS>(x.k[0], 2 * j + 1, s2[0], b2[0]);
+                    const uint32_t a3 = row_pair<T, BITS>(x.k[1], 2 * j + 1, s2[1], b2[1]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         if (j == 0) mma16816z<T>(sc[nt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
                         else mma16816<T>(sc[nt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    va[i][0] = cross_pair<T, BITS>(vw[0], vw[1], i, vsb[0][0], vsb[0][1]);
-                    va[i][1] = cross_pair<T, BITS>(vw[0], vw[1], MT + i, vsb[0][0], vsb[0][1]);
-                    va[i][2] = cross_pair<T, BITS>(vw[2], vw[3], i, vsb[1][0], vsb[1][1]);
-                    va[i][3] = cross_pair<T, BITS>(vw[2], vw[3], MT + i, vsb[1][0], vsb[1][1]);
-                }
             }
-            const bool ok0 = okk[0], ok1 = okk[1];
-            if (tile + 1 < te) load(tile + 1);
+            after_s();
             const bool plain = clean && k0 + 16 <= full;
             float grow = -INFINITY;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float x = sc[nt][e] * p.scale_log2;
+                    float y = sc[nt][e] * p.scale_log2;
                     if (!plain) {
                         const int key = k0 + r8 + 8 * (e >> 1), j = key - base;
-                        const bool see = key < kend && ((e >> 1) ? ok1 : ok0) &&
+                        const bool see = key < kend && (ok >> (e >> 1) & 1u) &&
                                          (j < 0 || (a.mask ? j < 64 && (vis[nt][e & 1] >> (j & 63) & 1)
                                                            : j <= qpos[nt][e & 1]));
-                        x = see ? x : -INFINITY;
+                        y = see ? y : -INFINITY;
                     }
-                    sc[nt][e] = x;
-                    grow = fmaxf(grow, x - m[nt][e & 1]);
+                    sc[nt][e] = y;
+                    grow = fmaxf(grow, y - m[nt][e & 1]);
                 }
             // The reference of the exponentials follows the running maximum only when a
             // score passes it by 2^8: the probabilities then reach 256, the sums lose nothing.
@@ -258,7 +270,7 @@ __global__ void __launch_bounds__(ra::THREADS)
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                         mx = fmaxf(mx, m[nt][e]);
-                        const float f = mx == -INFINITY ? 1.f : exp2f(m[nt][e] - mx);
+                        const float f = mx == -INFINITY ? 1.f : ex2(m[nt][e] - mx);
                         m[nt][e] = mx;
                         l[nt][e] *= f;
 #pragma unroll
@@ -268,20 +280,99 @@ __global__ void __launch_bounds__(ra::THREADS)
                         }
                     }
             }
+            uint32_t pb[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float pr[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float mr = m[nt][e & 1];
-                    pr[e] = exp2f(sc[nt][e] - (mr == -INFINITY ? 0.f : mr));
+                    pr[e] = ex2(sc[nt][e] - (mr == -INFINITY ? 0.f : mr));
                     l[nt][e & 1] += pr[e];
                 }
-                const uint32_t b0 = transpose8x8(pk_round<T>(pr[0], pr[1]));
-                const uint32_t b1 = transpose8x8(pk_round<T>(pr[2], pr[3]));
+                pb[nt][0] = transpose8x8(pk_round<T>(pr[0], pr[1]));
+                pb[nt][1] = transpose8x8(pk_round<T>(pr[2], pr[3]));
+            }
+            uint32_t s2[2] = {0u, 0u}, b2[2] = {0u, 0u};  // of value rows 2 c4, 2 c4 + 1; eight on
+            // values of keys that are not there multiply zeros: make them zeros
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    mma16816<T>(o[nt][i], va[i][0], va[i][1], va[i][2], va[i][3], b0, b1);
+            for (int h = 0; h < 2; ++h) {
+                uint32_t keep = 0xffffffffu;
+                if (!clean) {
+                    const int k = k0 + 8 * h + 2 * c4;
+                    const bool there = ok >> h & 1u;
+                    keep = (there && k < kend ? 0xffffu : 0u) | (there && k + 1 < kend ? 0xffff0000u : 0u);
+                }
+                if constexpr (BITS == 16) {
+                    if (!clean) {
+#pragma unroll
+                        for (int i = 0; i < HD / 16; ++i) {
+                            if (!(keep & 0xffffu)) x.v[2 * h][i] = 0u;
+                            if (!(keep >> 16)) x.v[2 * h + 1][i] = 0u;
+                        }
+                    }
+                } else {
+                    const uint32_t e0 = sb_of(x.vs, 8 * h + 2 * c4, vg), e1 = sb_of(x.vs, 8 * h + 2 * c4 + 1, vg);
+                    s2[h] = prmt(e0, e1, 0x5410u) & keep;
+                    b2[h] = prmt(e0, e1, 0x7632u) & keep;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint32_t a0 = cross_pair<T, BITS>(x.v[0], x.v[1], i, s2[0], b2[0]);
+                const uint32_t a1 = cross_pair<T, BITS>(x.v[0], x.v[1], MT + i, s2[0], b2[0]);
+                const uint32_t a2 = cross_pair<T, BITS>(x.v[2], x.v[3], i, s2[1], b2[1]);
+                const uint32_t a3 = cross_pair<T, BITS>(x.v[2], x.v[3], MT + i, s2[1], b2[1]);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+            }
+            after_pv();
+        };
+        auto nothing = [] {};
+
+        if (t0 < te) {
+            int pid[2];
+            uint32_t row[2];
+            pages(t0, pid);
+            uint32_t ok = rows(t0, pid, row);
+            Raw<HD, BITS> x;
+            load_k(x, row);
+            load_v(x, row);
+            pages(t0 + 1, pid);
+            if constexpr (BITS == 16) {
+                for (int tile = t0; tile < te; ++tile) {
+                    uint32_t ok1 = 0;
+                    tile_of(
+                        tile, x, ok,
+                        [&] {
+                            ok1 = rows(tile + 1, pid, row);
+                            if (tile + 1 < te) load_k(x, row);
+                            pages(tile + 2, pid);
+                        },
+                        [&] {
+                            if (tile + 1 < te) load_v(x, row);
+                        });
+                    ok = ok1;
+                }
+            } else {
+                Raw<HD, BITS> y;
+                for (int tile = t0; tile < te; tile += 2) {
+                    const uint32_t ok1 = rows(tile + 1, pid, row);
+                    if (tile + 1 < te) {
+                        load_k(y, row);
+                        load_v(y, row);
+                    }
+                    pages(tile + 2, pid);
+                    tile_of(tile, x, ok, nothing, nothing);
+                    if (tile + 1 >= te) break;
+                    ok = rows(tile + 2, pid, row);
+                    if (tile + 2 < te) {
+                        load_k(x, row);
+                        load_v(x, row);
+                    }
+                    pages(tile + 3, pid);
+                    tile_of(tile + 1, y, ok1, nothing, nothing);
+                }
             }
         }
 
@@ -317,7 +408,7 @@ __global__ void __launch_bounds__(ra::THREADS)
             for (int i = 0; i < WARPS; ++i) M = fmaxf(M, wm[i][row]);
 #pragma unroll
             for (int i = 0; i < WARPS; ++i) {
-                const float f = wm[i][row] == -INFINITY ? 0.f : exp2f(wm[i][row] - M);
+                const float f = wm[i][row] == -INFINITY ? 0.f : ex2(wm[i][row] - M);
                 den = fmaf(f, wl[i][row], den);
                 x = fmaf(f, wo[i][row][d], x);
                 y = fmaf(f, wo[i][row][d + 1], y);
@@ -354,12 +445,12 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
     float M = -INFINITY, den = 0.f, acc[DPL];
 #pragma unroll
     for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
-    for (int k0 = first; k0 <= c.last; k0 += AHEAD) {
+    for (int k0 = first; k0 <= c.last; k0 += AHEAD * c.step) {
         float2 ml[AHEAD];
         float v[AHEAD][DPL];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int k = min(k0 + i, c.last);
+            const int k = min(k0 + i * c.step, c.last);
             const size_t at = static_cast<size_t>(k == first ? c.slot : 2 * k) * ROWS + r;
             ml[i] = __ldcg(&p.part_ml[at]);
             if constexpr (DPL == 4) {
@@ -372,7 +463,7 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            if (k0 + i > c.last) break;
+            if (k0 + i * c.step > c.last) break;
             const float Mn = fmaxf(M, ml[i].x);
             const float co = M == -INFINITY ? 0.f : exp2f(M - Mn);
             const float cn = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - Mn);
@@ -399,7 +490,7 @@ namespace {
 // up to there, and from then on 128 of them as the M rows of tcgen05 products.
 struct Plan {
     bool tc;
-    int rows, kt, parts;
+    int rows, kt, parts, group;
 };
 Plan plan_of(const KvCache& c, const RowsArgs& a) {
     const long long r = static_cast<long long>(a.max_q) * (a.Hq / c.Hkv);
@@ -408,11 +499,17 @@ Plan plan_of(const KvCache& c, const RowsArgs& a) {
     p.rows = p.tc ? 128 : r > 8 ? 16 : 8;
     p.kt = p.tc ? kRowsTcKeys : ra::KT;
     // CTAs the units are shared out to: what the GPU holds at once, at most one per unit
-    const long long most = 148LL * (p.rows == 8 ? 4 : 2);
+    const long long most = 148LL * (p.tc ? 2 : ra::resident(c.hd, c.bits, p.rows / 8));
     const long long tiles = (a.max_kv + p.kt - 1) / p.kt;
     long long units = (r + p.rows - 1) / p.rows * (tiles > 0 ? tiles : 1) * c.Hkv;
     units = units < most ? units * a.batch : most;
     p.parts = static_cast<int>(units < 1 ? 1 : units < most ? units : most);
+    // up to eight chunks go side by side
+    const int chunks = static_cast<int>((r + p.rows - 1) / p.rows);
+    p.group = p.tc && chunks >= 2 && chunks <= 8 ? chunks : 1;
+    if (p.group > 1) p.parts = (p.parts + p.group - 1) / p.group * p.group > most
+                                   ? static_cast<int>(most / p.group * p.group)
+                                   : (p.parts + p.group - 1) / p.group * p.group;
     return p;
 }
 
@@ -475,6 +572,7 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& all, void* worksp
     p.c = c;
     p.scale_log2 = all.scale * 1.4426950408889634f;
     p.parts = pl.parts;
+    p.group = pl.group;
     char* ws = static_cast<char*>(workspace);
     p.part_o = reinterpret_cast<float*>(ws);
     ws += round256(rows * c.hd * sizeof(float));

@@ -64,11 +64,6 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ float ex2(float x) {  // 2^x, results below 2^-126 as zero
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
-    return r;
-}
 
 // 3-D TMA load of one box (64 dims, one head, some rows); no cluster multicast.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
@@ -139,14 +134,14 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     const KvCache& c = p.c;
     const int Hkv = c.Hkv, G = a.Hq / Hkv;
     zero_tail(a, HD, THREADS);
-    const Units un = scan_units<KT>(a, Hkv, G, ROWS, pref);
+    const Units un = scan_units<KT>(a, Hkv, G, ROWS, p.group, pref);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int page_shift = 31 - __clz(c.page);
     Walk<KT, ROWS> w;
-    w.begin(a, Hkv, un, p.parts, pref);
+    w.begin(a, Hkv, un, p.parts, p.group, pref);
 
     // Tile j of the CTA's run uses buffer j & 1 of K, V, S and P, and that buffer's barriers'
     // phase j >> 1; item i the queries' barriers' phase i. No role is ever two phases behind
@@ -496,29 +491,57 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
 }
 
 // The values of every sequence's keys, from the first to the end of its last tile (zeros
-// behind the last key and for pages outside the pool): block (eight keys, sequence, keys or
-// values), thread = eight dims of a head at a time. Eight keys share a page.
+// behind the last key and for pages outside the pool): block (tile of 64 keys, sequence,
+// keys or values), thread = 16 bytes of codes at a time, four of them in flight.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
     kv_expand_kernel(const KvCache c, const RowsArgs a, int rows_per_seq, T* __restrict__ k_out,
                      T* __restrict__ v_out) {
+    constexpr int CPU = 16 / BITS, AHEAD = 4;  // chunks of eight values in 16 bytes
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.y, cpr = c.Hkv * c.hd / 8, key = blockIdx.x * 8;
+    const bool is_v = blockIdx.z != 0;
+    const int b = blockIdx.y, k0 = blockIdx.x * rt::KT;
     const int L = max(0, min(a.kv_lens[b], a.max_kv));
-    if (key >= (L + rt::KT - 1) / rt::KT * rt::KT) return;
-    int pid = -1;
-    if (key < L) pid = __ldg(a.table + static_cast<size_t>(b) * a.max_blocks + key / c.page);
-    const bool there = pid >= 0 && pid < c.pages;
-    const size_t from = there ? (static_cast<size_t>(pid) * c.page + key % c.page) * cpr : 0;
-    uint4* out = reinterpret_cast<uint4*>(blockIdx.z ? v_out : k_out) +
-                 (static_cast<size_t>(b) * rows_per_seq + key) * cpr;
-    const int n = there ? min(8, L - key) * cpr : 0;  // chunks that hold values
-#pragma unroll 4
-    for (int i = threadIdx.x; i < 8 * cpr; i += 256) {
-        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-        if (i < n) o = cache_chunk<T, BITS>(c, blockIdx.z != 0, from + i);
-        out[i] = o;
+    if (k0 >= L) return;
+    const int upr = c.Hkv * c.hd * BITS / 128, units = rt::KT * upr;  // of 16 bytes, in a row
+    const int32_t* bt = a.table + static_cast<size_t>(b) * a.max_blocks;
+    const int page_shift = 31 - __clz(c.page), gpu = 128 / BITS;     // (elements of a unit)
+    const uint4* codes = static_cast<const uint4*>(is_v ? c.v : c.k);
+    const uint16_t* sp = static_cast<const uint16_t*>(is_v ? c.vs : c.ks);
+    const uint16_t* bp = static_cast<const uint16_t*>(is_v ? c.vb : c.kb);
+    uint4* out = reinterpret_cast<uint4*>(is_v ? v_out : k_out) +
+                 (static_cast<size_t>(b) * rows_per_seq + k0) * upr * CPU;
+    for (int i0 = threadIdx.x; i0 < units; i0 += 256 * AHEAD) {
+        uint4 raw[AHEAD];
+        uint32_t s[AHEAD], z[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * 256, row = i / upr, key = k0 + row;
+            raw[j] = make_uint4(0u, 0u, 0u, 0u);
+            s[j] = z[j] = 0u;
+            if (i < units && key < L) {
+                const int pid = __ldg(bt + (key >> page_shift));
+                if (pid >= 0 && pid < c.pages) {
+                    const size_t at = ((static_cast<size_t>(pid) << page_shift) + (key & (c.page - 1))) * upr +
+                                      (i - row * upr);
+                    raw[j] = __ldg(codes + at);
+                    const size_t g = at * gpu / c.gs;
+                    s[j] = __ldg(sp + g);
+                    z[j] = __ldg(bp + g);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = i0 + j * 256;
+            if (i >= units) break;
+            const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+            for (int q = 0; q < CPU; ++q)
+                out[static_cast<size_t>(i) * CPU + q] =
+                    in_order<T, BITS>(w + q * (BITS / 4), pk_splat(s[j]), pk_splat(z[j]));
+        }
     }
 }
 
@@ -585,7 +608,7 @@ cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStre
                                           : reinterpret_cast<const void*>(&kv_expand_kernel<__half, 4>));
         static PerDevice cfg[4];
         const cudaError_t e = launch_ex(f, cfg[(bf ? 0 : 2) + (c.bits == 8 ? 0 : 1)],
-                                        dim3(rps / 8, p.a.batch, 2), dim3(256), 0, st, overlap, args);
+                                        dim3(rps / rt::KT, p.a.batch, 2), dim3(256), 0, st, overlap, args);
         if (e != cudaSuccess) return e;
         overlap = true;  // (the attention waits for the whole of it)
         k = ko;

@@ -1,7 +1,11 @@
 // How attention over pages shares its work out: the query rows of every (sequence, kv head)
 // in chunks, each chunk's keys in tiles, and the tiles of all (sequence, chunk, kv head)
-// items as one sequence of units that the CTAs take in equal contiguous runs. And how the
-// parts of an item that several CTAs computed are joined.
+// items as one sequence of units that the CTAs take in equal contiguous runs. Or, with few
+// chunks (a tree's), the tiles of all (sequence, kv head) items, of which C CTAs take the
+// same run, each another chunk: they read the same keys at about the same time, so that all
+// but one find them in L2 (16 trees of 64 tokens over 8192 16-bit keys, 448 rows in four
+// chunks over 168 MB: 127 us with the chunks as units of their own). And how the parts of an item that
+// several CTAs computed are joined.
 #pragma once
 
 #include "common.cuh"
@@ -11,11 +15,11 @@ namespace mlxq {
 namespace ra {
 
 // An item whose tiles several CTAs took, recorded by the CTA that took the first of them:
-// its partial results are in that CTA's slot `slot`, then in slot 0 of the CTAs up to
-// `last`, in order of keys.
+// its partial results are in that CTA's slot `slot`, then in slot 0 of every step-th CTA up
+// to `last`, in order of keys.
 struct Cut {
     int rows;   // rows of the chunk (0: this CTA began no such item)
-    int slot, last;
+    int slot, last, step;
     int row0, rr0, g;  // the sequence's first row of q, the chunk's first row, the kv head
 };
 
@@ -26,7 +30,8 @@ struct Params {
     float* part_o;    // [2 P][ROWS][HD] unnormalised outputs
     float2* part_ml;  // [2 P][ROWS] maximum (base 2) and sum
     Cut* cut;         // [P]
-    int parts;        // P: CTAs the units are shared out to
+    int parts;        // P: CTAs, of which each run of `group` takes the same units
+    int group;        // C: 1, or the most chunks of a sequence, each CTA of the run one of them
 };
 
 // One sequence's place in the batch, with everything a bad length or offset could do bounded.
@@ -57,7 +62,7 @@ struct Units {
     int per;  // sequences per scanning thread
 };
 template <int KT>
-__device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, int rows,
+__device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, int rows, int group,
                                             int* pref /* shared [SCAN + 1] */) {
     __shared__ int wsum[SCAN / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -67,7 +72,7 @@ __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, i
     if (tid < SCAN) {
         for (int b = tid * u.per; b < min(a.batch, (tid + 1) * u.per); ++b) {
             const Seq s = seq_of<KT>(a, b, G, rows);
-            inc += s.chunks * s.tiles * Hkv;
+            inc += (group > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -92,16 +97,18 @@ __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, i
 template <int KT, int ROWS>
 struct Walk {
     int u, u_lo, u_hi, start;
-    int b, G, Hkv, share, extra;
+    int b, G, Hkv, share, extra, C, ch;
     // the segment
     Seq s;
     int g, rr0, t0, t1;
 
     __device__ __forceinline__ void begin(const RowsArgs& a, int Hkv_, const Units& un, int parts,
-                                          const int* pref) {
+                                          int group, const int* pref) {
         Hkv = Hkv_;
         G = a.Hq / Hkv;
-        const int P = max(1, min(parts, un.total)), i = blockIdx.x;  // no share is empty
+        C = group;
+        const int P = max(1, min(parts / C, un.total)), i = blockIdx.x / C;  // no share is empty
+        ch = blockIdx.x - i * C;
         share = un.total / P;
         extra = un.total - share * P;
         u = u_lo = u_hi = start = b = 0;
@@ -121,19 +128,30 @@ struct Walk {
     __device__ __forceinline__ bool next(const RowsArgs& a) {
         while (u < u_hi) {
             s = seq_of<KT>(a, b, G, ROWS);
-            const int n = s.chunks * s.tiles * Hkv;
+            const int n = (C > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
             if (u >= start + n) {
                 start += n;
                 ++b;
                 continue;
             }
-            // kv head fastest outside the tiles: neighbouring runs read neighbouring parts
-            // of the same pages
+            if (C > 1 && ch >= s.chunks) {  // no rows of this sequence for this CTA
+                u = min(u_hi, start + n);
+                continue;
+            }
             const int item = (u - start) / s.tiles;
             t0 = (u - start) - item * s.tiles;
             t1 = min(s.tiles, t0 + (u_hi - u));
-            g = item % Hkv;
-            rr0 = item / Hkv * ROWS;
+            int chunk = ch;
+            g = item;
+            if (C == 1) {
+                // The chunks in pairs from both ends: a causal mask leaves the first ones
+                // fewer keys than the last, and a run of items then has its share of both
+                const int pair = item / (2 * Hkv), in = item - pair * 2 * Hkv;
+                const bool lone = 2 * pair + 1 == s.chunks;
+                g = lone ? in : in >> 1;
+                chunk = !lone && (in & 1) ? s.chunks - 1 - pair : pair;
+            }
+            rr0 = chunk * ROWS;
             return true;
         }
         return false;
@@ -152,7 +170,7 @@ struct Walk {
     __device__ __forceinline__ int tile_end(const RowsArgs& a) const {
         return min(t1, (kend(a) + KT - 1) / KT);
     }
-    // The CTA that owns unit x.
+    // The CTA (run of CTAs) that owns unit x.
     __device__ __forceinline__ int owner(int x) const {
         const int big = extra * (share + 1);
         return x < big ? x / (share + 1) : extra + (x - big) / share;
@@ -161,7 +179,8 @@ struct Walk {
         Cut c;
         c.rows = min(s.n * G - rr0, ROWS);
         c.slot = slot();
-        c.last = owner(u - t0 + s.tiles - 1);
+        c.last = owner(u - t0 + s.tiles - 1) * C + ch;
+        c.step = C;
         c.row0 = s.row0;
         c.rr0 = rr0;
         c.g = g;
