@@ -15,8 +15,9 @@
 //               memory as it lies (key rows, dimensions contiguous)
 // S, K and V have two buffers each, so S of the next tile is there when the softmax of this
 // one ends, and P V runs under the next softmax. Warps 0-3 hold a tensor-memory lane quarter
-// each and do the softmax and the epilogue; warp 4 brings keys and values in by TMA, a box
-// to a page; a thread of warp 5 issues the products; warps 6 and 7 bring the queries of the
+// each and do the softmax and the epilogue; warp 4 brings keys in by TMA and warp 6 values, a
+// box to a page and 64 dims (one warp for both takes 2100 cycles a tile of 16-key pages,
+// longer than the softmax); warp 5 issues the products; warp 7 brings the queries of the
 // next item. Two CTAs share an SM (96 KB of shared memory and 256 columns each).
 // Work is shared out as in rows_units.cuh. Every wait is bounded: on a timeout the CTA
 // records an error, its roles stop, what is in flight is waited for, tensor memory is
@@ -38,7 +39,7 @@ __device__ int g_rows_tc_error;  // 0, or the first error code a kernel recorded
 
 namespace rt {
 constexpr int ROWS = 128, KT = kRowsTcKeys, THREADS = kRowsTcThreads;
-constexpr int WARP_TMA = 4, WARP_MMA = 5, WARP_Q0 = 6;
+constexpr int WARP_K = 4, WARP_MMA = 5, WARP_V = 6;  // and 7: queries
 constexpr uint32_t kCols = 256;   // tensor memory: S (and P) from 0 and 64, O from 128
 constexpr uint32_t kOCol = 128;
 constexpr uint32_t kParkNs = 2000, kParkLimit = 1u << 20;  // ~2 s
@@ -118,17 +119,15 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             mbar_init(smem_u32(s_full + i), 1);
             mbar_init(smem_u32(pv_done + i), 1);
         }
-        mbar_init(smem_u32(&q_full), 2);
+        mbar_init(smem_u32(&q_full), 1);
         mbar_init(smem_u32(&q_free), 1);
         mbar_init(smem_u32(&v_land), 1);
         mbar_init(smem_u32(&drained), 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == WARP_TMA && lane == 0) {
-        tma_prefetch_map(&tk);
-        tma_prefetch_map(&tv);
-    }
+    if (warp == WARP_K && lane == 0) tma_prefetch_map(&tk);
+    if (warp == WARP_V && lane == 0) tma_prefetch_map(&tv);
     pdl_wait();
     const RowsArgs& a = p.a;
     const KvCache& c = p.c;
@@ -174,95 +173,91 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         return false;
     };
 
-    if (warp == WARP_TMA) {
-        // ------------------------------ keys and values ------------------------------
+    if (warp == WARP_K || warp == WARP_V) {
+        // ------------------------------ keys, values ---------------------------------
         // lane = (box of the tile, 64-dim half); a box that is not there is read from behind
         // the source's last row, which gives zeros
+        const bool is_v = warp == WARP_V;
+        const CUtensorMap* map = is_v ? &tv : &tk;
+        uint64_t *full = is_v ? v_full : k_full, *freed = is_v ? pv_done : s_full;
+        uint8_t* tiles = is_v ? vs : ks;
         const int nbox = KT / src.box, half = lane % HALVES, box = lane / HALVES;
         const bool loads = box < nbox;
         const uint32_t off = static_cast<uint32_t>(half * (KT * 128) + box * src.box * 128);
-        auto row_of = [&]() -> int {
+        auto page_of = [&]() -> int {  // (loaded a tile before it is used)
             const int key = tile * KT + box * src.box;
-            if (!loads || key >= kend) return src.rows;
+            if (!loads || key >= kend) return -1;
             if (src.rows_per_seq) return w.b * src.rows_per_seq + key;
-            const int pid = __ldg(a.table + static_cast<size_t>(w.b) * a.max_blocks + (key >> page_shift));
-            return pid >= 0 && pid < c.pages ? (pid << page_shift) : src.rows;
+            return __ldg(a.table + static_cast<size_t>(w.b) * a.max_blocks + (key >> page_shift));
         };
         uint32_t j = 0, lands = 0;
         bool more = step();
-        int row = more ? row_of() : 0;
+        int page = more ? page_of() : -1;
         for (; more; ++j) {
-            const int g = w.g, now = row, left = kend - tile * KT;  // keys of the tile
-            if (j > 1 && !wait(s_full, j - 2)) break;
-            const uint32_t kb = smem_u32(k_full + (j & 1)), vb = smem_u32(v_full + (j & 1));
-            if (lane == 0) mbar_arrive_expect_tx(kb, HB);
-            __syncwarp();
-            if (loads) tma_load_3d(smem_u32(ks + (j & 1) * HB) + off, &tk, kb, half * 64, g, now);
+            const int g = w.g, left = kend - tile * KT;  // keys of the tile
+            const int row = page < 0 ? src.rows
+                            : src.rows_per_seq ? page
+                            : page < c.pages   ? page << page_shift
+                                               : src.rows;
             more = step();
-            if (more) row = row_of();
-            if (j > 1 && !wait(pv_done, j - 2)) break;
-            uint8_t* v = vs + (j & 1) * HB;
-            // A page's rows behind the last key hold anything, and its probability of zero
-            // does not make a number of what is none: those rows are zeroed once they landed.
-            const bool ragged = left < KT && (left & (src.box - 1)) && !src.rows_per_seq;
-            const uint32_t to = ragged ? smem_u32(&v_land) : vb;
+            page = more ? page_of() : -1;
+            if (j > 1 && !wait(freed, j - 2)) {
+                more = true;
+                break;
+            }
+            uint8_t* dst = tiles + (j & 1) * HB;
+            const uint32_t bar = smem_u32(full + (j & 1));
+            // A page's rows behind the last key hold anything, and a probability of zero does
+            // not make a number of what is none: those rows of V are zeroed once they landed.
+            const bool ragged = is_v && left < KT && (left & (src.box - 1)) && !src.rows_per_seq;
+            const uint32_t to = ragged ? smem_u32(&v_land) : bar;
             if (lane == 0) mbar_arrive_expect_tx(to, HB);
             __syncwarp();
-            if (loads) tma_load_3d(smem_u32(v) + off, &tv, to, half * 64, g, now);
+            if (loads) tma_load_3d(smem_u32(dst) + off, map, to, half * 64, g, row);
             if (ragged) {
-                if (!wait_at(&v_land, lands++)) break;
+                if (!wait_at(&v_land, lands++)) {
+                    more = true;
+                    break;
+                }
                 const int end = min(KT, (left + src.box - 1) & ~(src.box - 1));
                 for (int i = left * 8 + lane; i < end * 8; i += 32)
 #pragma unroll
                     for (int h = 0; h < HALVES; ++h)
-                        *reinterpret_cast<uint4*>(v + h * (KT * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(dst + h * (KT * 128) + i * 16) = make_uint4(0u, 0u, 0u, 0u);
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(vb);
+                if (lane == 0) mbar_arrive(bar);
             }
         }
         if (more) {  // stopped early: the copies under way land before the CTA ends
-            for (uint32_t i = j > 1 ? j - 2 : 0; i <= j; ++i) {
-                mbar_wait_bounded(smem_u32(k_full + (i & 1)), (i >> 1) & 1, kSpinLimit);
-                mbar_wait_bounded(smem_u32(v_full + (i & 1)), (i >> 1) & 1, kSpinLimit);
-            }
+            for (uint32_t i = j > 1 ? j - 2 : 0; i < j; ++i)
+                mbar_wait_bounded(smem_u32(full + (i & 1)), (i >> 1) & 1, kSpinLimit);
             if (lands) mbar_wait_bounded(smem_u32(&v_land), (lands - 1) & 1, kSpinLimit);
         }
-    } else if (warp >= WARP_Q0) {
+    } else if (warp > WARP_V) {
         // ------------------------------ queries --------------------------------------
-        constexpr int QL = HD / 8, RPI = 32 / QL, QB = 16;  // lanes of a row, rows and loads at once
-        const bool neg = p.scale_log2 < 0.f;  // the sign of the scale goes into the queries
-        const int inv = 65536 / G + 1;        // t / G = t * inv >> 16 for t < 136
+        constexpr int QL = HD / 8, RPI = 32 / QL;  // lanes of a row, rows at once
+        const int inv = 65536 / G + 1;             // t / G = t * inv >> 16 for t < 136
         uint32_t item = 0;
         for (; w.next(a); w.advance()) {
             if (w.tile_end(a) <= w.t0) continue;
             if (item > 0 && !wait_at(&q_free, item - 1)) break;  // the last S of the item before
             ++item;
-            const int R = w.s.n * G, n0 = w.rr0 / G, h0 = w.rr0 - n0 * G;
-            const int r0 = (warp - WARP_Q0) * 64 + lane / QL, ch = lane % QL;
+            const int R = w.s.n * G, n0 = w.rr0 / G, h0 = w.rr0 - n0 * G, ch = lane % QL;
             const T* q = static_cast<const T*>(a.q) +
                          (static_cast<size_t>(w.s.row0 + n0) * a.Hq + w.g * G) * HD + ch * 8;
-#pragma unroll 1
-            for (int i0 = 0; i0 < 64 / RPI; i0 += QB) {
-                uint4 v[QB];
-#pragma unroll
-                for (int i = 0; i < QB; ++i) {
-                    const int r = r0 + (i0 + i) * RPI, t = h0 + r, dn = t * inv >> 16;
-                    v[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (w.rr0 + r < R)
-                        v[i] = *reinterpret_cast<const uint4*>(
-                            q + (static_cast<size_t>(dn) * a.Hq + t - dn * G) * HD);
-                }
-                const uint32_t sign = neg ? 0x80008000u : 0u;
-#pragma unroll
-                for (int i = 0; i < QB; ++i) {
-                    const int r = r0 + (i0 + i) * RPI;
-                    // rows of 128 bytes, sixteen-byte chunks swizzled, a half after the other
-                    *reinterpret_cast<uint4*>(qs + (ch / 8) * (ROWS * 128) + r * 128 +
-                                              (((ch % 8) ^ (r & 7)) << 4)) =
-                        make_uint4(v[i].x ^ sign, v[i].y ^ sign, v[i].z ^ sign, v[i].w ^ sign);
-                }
+#pragma unroll 8
+            for (int r = lane / QL; r < ROWS; r += RPI) {
+                const int t = h0 + r, dn = t * inv >> 16;
+                const bool in = w.rr0 + r < R;
+                // rows of 128 bytes, sixteen-byte chunks swizzled, a half after the other
+                cp_async16(qs + (ch / 8) * (ROWS * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4),
+                           in ? q + (static_cast<size_t>(dn) * a.Hq + t - dn * G) * HD
+                              : static_cast<const T*>(a.q),
+                           in ? 16 : 0);
             }
+            cp_async_commit();
+            cp_async_wait<0>();
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&q_full));
@@ -366,6 +361,10 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
                 if (some) {
                     uint32_t v[2][32];
                     tmem_ld64(t_s, v[0], v[1]);
+                    if (p.scale_log2 < 0.f) {  // the sign of the scale goes into the scores
+#pragma unroll
+                        for (int x = 0; x < 64; ++x) v[x / 32][x % 32] ^= 0x80000000u;
+                    }
                     if (!clean) {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
