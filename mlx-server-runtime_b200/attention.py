@@ -111,30 +111,39 @@ def _kv_struct(k, v) -> _lib.KVCache:
                             k.biases.data_ptr(), v.scales.data_ptr(), v.biases.data_ptr(), pages,
                             page, hkv, k.scales.shape[3] * k.group_size, k.bits, k.group_size,
                             _DT[k.dtype])
-    if isinstance(v, QuantizedKV) or k.shape != v.shape or k.dtype != v.dtype:
+    shape, dt = k.shape, k.dtype
+    if isinstance(v, QuantizedKV) or v.shape != shape or v.dtype is not dt:
         raise ValueError("k_cache and v_cache must share shape and dtype")
-    if k.ndim != 4 or not k.is_contiguous() or not v.is_contiguous():
+    if len(shape) != 4 or not k.is_contiguous() or not v.is_contiguous():
         raise ValueError("caches must be contiguous [pages, page_size, n_kv_heads, head_dim]")
-    pages, page, hkv, hd = k.shape
-    return _lib.KVCache(k.data_ptr(), v.data_ptr(), None, None, None, None, pages, page, hkv, hd,
-                        16, 0, _code(k, "the cache"))
+    if dt not in _DT:
+        raise ValueError(f"the cache must be bfloat16 or float16, got {dt}")
+    return _lib.KVCache(k.data_ptr(), v.data_ptr(), None, None, None, None, *shape, 16, 0, _DT[dt])
 
 
-def _on(dev: torch.device, *ts) -> None:
-    """Every tensor on the CUDA device `dev`."""
-    if dev.type != "cuda":
-        raise ValueError(f"expected CUDA tensors, got a tensor on {dev}")
-    for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors are on different devices ({dev} and {t.device})")
+def _on(t: torch.Tensor, *ts) -> int:
+    """The index of t's CUDA device, which every other tensor has to be on."""
+    i = t.get_device()
+    if i < 0:
+        raise ValueError(f"expected CUDA tensors, got a tensor on {t.device}")
+    for u in ts:
+        if u is not None and u.get_device() != i:
+            raise ValueError(f"tensors are on different devices ({t.device} and {u.device})")
+    return i
 
 
-def _call(dev: torch.device, call):
-    """call(stream) with `dev` current, on its current stream."""
-    if torch.cuda.current_device() == dev.index:
-        return call(_stream(dev))
-    with torch.cuda.device(dev):
-        return call(_stream(dev))
+def _call(i: int, call):
+    """call(stream) with device i current, on its current stream. (The raw handle: making
+    a Stream object takes longer than a small launch.)"""
+    if torch._C._cuda_getDevice() == i:
+        return call(torch._C._cuda_getCurrentRawStream(i))
+    with torch.cuda.device(i):
+        return call(torch._C._cuda_getCurrentRawStream(i))
+
+
+def _pool(c) -> torch.Tensor:
+    """A tensor of a cache side, for its device."""
+    return c.codes if isinstance(c, QuantizedKV) else c
 
 
 def _i32(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -209,28 +218,30 @@ def rope_kv_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tens
 def _norm_rope_append(qkv, positions, slots, k_cache, v_cache, n_heads, n_kv_heads, head_dim,
                       base, q_norm, k_norm, eps):
     kv = _kv_struct(k_cache, v_cache)
-    if qkv.ndim != 2 or qkv.stride(1) != 1 or qkv.dtype != k_cache.dtype:
+    dt = qkv.dtype
+    if qkv.dim() != 2 or qkv.stride(1) != 1 or dt is not k_cache.dtype:
         raise ValueError("qkv must be a 2-D tensor with contiguous rows, of the caches' dtype")
     if kv.n_kv_heads != n_kv_heads or kv.head_dim != head_dim:
         raise ValueError("caches must hold n_kv_heads heads of head_dim")
-    T = qkv.shape[0]
-    if n_heads <= 0 or qkv.shape[1] < (n_heads + 2 * n_kv_heads) * head_dim:
+    T, width = qkv.shape
+    if n_heads <= 0 or width < (n_heads + 2 * n_kv_heads) * head_dim:
         raise ValueError("qkv's rows must hold q, k and v")
     for w in (q_norm, k_norm):
-        if w is not None and (w.shape != (head_dim,) or w.dtype != qkv.dtype or
+        if w is not None and (w.dim() != 1 or w.numel() != head_dim or w.dtype is not dt or
                               not w.is_contiguous()):
-            raise ValueError(f"norm weights must be contiguous [{head_dim}] of dtype {qkv.dtype}")
+            raise ValueError(f"norm weights must be contiguous [{head_dim}] of dtype {dt}")
     positions, slots = _i32(positions, "positions"), _i32(slots, "slots")
-    if positions.shape != (T,) or slots.shape != (T,):
+    if positions.dim() != 1 or positions.numel() != T or slots.dim() != 1 or slots.numel() != T:
         raise ValueError(f"positions and slots must be [{T}]")
-    dev = qkv.device
-    _on(dev, positions, slots, k_cache, v_cache, q_norm, k_norm)
-    q = torch.empty(T, n_heads, head_dim, dtype=qkv.dtype, device=dev)
+    dev = _on(qkv, positions, slots, _pool(k_cache), _pool(v_cache), q_norm, k_norm)
+    q = qkv.new_empty((T, n_heads, head_dim))
     # (a single row's stride is arbitrary)
-    ld = qkv.stride(0) if T > 1 else (qkv.shape[1] + 7) // 8 * 8
-    rc = _call(dev, lambda st: _lib.load().mlxq_norm_rope_kv_append(
-        kv, _p(qkv), ld, _p(q), _p(q_norm), _p(k_norm), float(eps), _p(positions), _p(slots), T,
-        n_heads, float(base), st))
+    ld = qkv.stride(0) if T > 1 else (width + 7) // 8 * 8
+    append = _lib.load().mlxq_norm_rope_kv_append
+    rc = _call(dev, lambda st: append(
+        kv, qkv.data_ptr(), ld, q.data_ptr(), None if q_norm is None else q_norm.data_ptr(),
+        None if k_norm is None else k_norm.data_ptr(), eps, positions.data_ptr(),
+        slots.data_ptr(), T, n_heads, base, st))
     _lib.check(rc, "rope_kv_append")
     return q
 
@@ -243,11 +254,10 @@ def kv_cache_read(k_cache, v_cache, slots: torch.Tensor):
     slots = _i32(slots, "slots")
     if slots.ndim != 1:
         raise ValueError("slots must be [n]")
-    dev = k_cache.device
-    _on(dev, v_cache, slots)
+    dev = _on(_pool(k_cache), _pool(v_cache), slots)
     n = slots.shape[0]
-    k, v = (torch.empty(n, kv.n_kv_heads, kv.head_dim, dtype=k_cache.dtype, device=dev)
-            for _ in range(2))
+    values = k_cache.scales if kv.bits != 16 else k_cache
+    k, v = (values.new_empty((n, kv.n_kv_heads, kv.head_dim)) for _ in range(2))
     rc = _call(dev, lambda st: _lib.load().mlxq_kv_cache_read(kv, _p(slots), n, _p(k), _p(v), st))
     _lib.check(rc, "kv_cache_read")
     return k, v
@@ -274,22 +284,22 @@ def _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, 
         if tree_mask.dtype != torch.int64 or tree_mask.shape != (q.shape[0],):
             raise ValueError(f"tree_mask must be int64 [{q.shape[0]}]")
         tree_mask = tree_mask.contiguous()
-    dev = q.device
-    _on(dev, cu_q, k_cache, v_cache, block_table, kv_lens, tree_mask)
+    dev = _on(q, cu_q, _pool(k_cache), _pool(v_cache), block_table, kv_lens, tree_mask)
     out = torch.empty_like(q)
-    L = _lib.load()
     rows, H, _ = q.shape
     max_q_len, max_kv_len = int(max_q_len), int(max_kv_len)
+    L = _lib.load()
 
     def call(st):
         need = L.mlxq_paged_attention_rows_workspace_size(kv, B, max_q_len, max_kv_len, H)
         # per call, from the allocator: calls on other streams and in other captured graphs
         # have their own
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        return L.mlxq_paged_attention_rows(kv, _p(q), _p(cu_q), rows, max_q_len, _p(block_table),
-                                           block_table.shape[1], _p(kv_lens), max_kv_len,
-                                           _p(tree_mask), _p(out), B, H, float(scale), _p(ws),
-                                           need, st)
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        return L.mlxq_paged_attention_rows(
+            kv, q.data_ptr(), None if cu_q is None else cu_q.data_ptr(), rows, max_q_len,
+            block_table.data_ptr(), block_table.shape[1], kv_lens.data_ptr(), max_kv_len,
+            None if tree_mask is None else tree_mask.data_ptr(), out.data_ptr(), B, H,
+            float(scale), None if ws is None else ws.data_ptr(), need, st)
 
     _lib.check(_call(dev, call), what)
     return out
