@@ -32,7 +32,7 @@ namespace mlxq {
 
 namespace ra {
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int KT = 16 * WARPS;  // keys per tile
+constexpr int KT = 32 * WARPS;  // keys per tile
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -62,26 +62,19 @@ __device__ __forceinline__ void ldw(const void* at, uint32_t (&r)[N]) {
 
 // CTAs of an SM: what the registers of a variant allow (and the launch bounds ask for).
 constexpr int resident(int hd, int bits, int nt) {
-    return nt == 2 ? 2 : hd == 64 ? 4 : bits == 4 ? 4 : bits == 8 ? 3 : 2;
+    return nt == 2 ? 2 : bits == 16 ? (hd == 64 ? 3 : 2) : hd == 64 || bits == 4 ? 4 : 3;
 }
-
-// A lane's part of 16 keys on its way: words of key rows r8 and r8 + 8 (a quarter of each),
-// of value rows 2 c4, 2 c4 + 1 and eight on (an eighth of each); and of (key lane % 16,
-// group lane / 16, and with four groups lane / 16 + 2) scale | bias << 16.
-template <int HD, int BITS>
-struct Raw {
-    uint32_t k[2][HD / 4 * BITS / 32], v[4][HD / 8 * BITS / 32];
-    uint32_t ks[2], vs[2];
-};
 }  // namespace ra
 
-template <typename T, int HD, int BITS, int NT>
+// NG: quantisation groups of a head's row (1 for 16-bit rows).
+template <typename T, int HD, int BITS, int NG, int NT>
 __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
     attn_rows_kernel(const __grid_constant__ ra::Params p) {
     using namespace ra;
     constexpr int ROWS = 8 * NT;
     constexpr int RB = HD * BITS / 8;  // bytes of a row
     constexpr int MT = HD / 16;
+    constexpr int KW = HD / 4 * BITS / 32, VW = HD / 8 * BITS / 32;  // a lane's words of a row
     __shared__ int pref[SCAN + 1];
     __shared__ float wo[WARPS][ROWS][HD + 4];
     __shared__ float wm[WARPS][ROWS], wl[WARPS][ROWS];
@@ -101,9 +94,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
     w.begin(a, Hkv, un, p.parts, p.group, pref);
     Cut mine = {};
 
-    const int ng = BITS == 16 ? 1 : HD / c.gs;
-    const int kg = BITS == 16 ? 0 : c4 * (HD / 4) / c.gs;  // this lane's group of a key row
-    const int vg = BITS == 16 ? 0 : r8 * (HD / 8) / c.gs;  // and of a value row
+    const int kg = NG == 1 ? 0 : c4 * NG / 4;  // this lane's group of a key row
+    const int vg = NG == 1 ? 0 : r8 * NG / 8;  // and of a value row
     const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * RB;  // of a token: its heads' rows
 
     for (; w.next(a); w.advance()) {
@@ -111,6 +103,72 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
         const int g = w.g, row_lo = w.rr0, t0 = w.t0, R = s.n * G;
         const int base = w.base(), kend = w.kend(a), full = min(max(base, 0), kend);
         const int32_t* bt = a.table + static_cast<size_t>(w.b) * a.max_blocks;
+        const int te = w.tile_end(a);
+
+        // A warp takes 32 keys of each tile, lane = key of them for the page ids. Eight keys
+        // share a page: eight e of the 32 begins at the row lane 8 e holds; -1: not there.
+        // Page ids are loaded two steps before their use, rows one.
+        auto page_id = [&](int tile) -> int {
+            const int key = tile * KT + warp * 32 + lane;
+            return tile < te && key < kend ? __ldg(bt + (key >> page_shift)) : -1;
+        };
+        auto row_id = [&](int tile, int pid) -> uint32_t {
+            if (pid < 0 || pid >= c.pages) return ~0u;
+            return (static_cast<uint32_t>(pid) << page_shift) +
+                   (static_cast<uint32_t>(tile * KT + warp * 32 + lane) & (c.page - 1));
+        };
+        // A row that is not there is read from row 0 of the pool (and not used).
+        auto row_at = [&](uint32_t rows, int key) -> size_t {
+            const uint32_t r = __shfl_sync(0xffffffffu, rows, key);
+            return r == ~0u ? 0 : r;
+        };
+        // Words of key rows r8 and r8 + 8 of each sixteen (a quarter of each), of value rows
+        // 2 c4, 2 c4 + 1 and eight on (an eighth of each); of 32 keys x NG groups in order,
+        // NG to a lane: scales and biases.
+        uint32_t kw[2][2][KW], vw[2][4][VW];
+        uint16_t ks[NG], kb[NG], vs[NG], vb[NG];
+        auto load_k = [&](uint32_t rows) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    ldw(static_cast<const char*>(c.k) + row_at(rows, 16 * mt + 8 * h + r8) * row_bytes +
+                            g * RB + c4 * (RB / 4),
+                        kw[mt][h]);
+            if constexpr (BITS != 16) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const int id = 32 * i + lane;
+                    const size_t at = (row_at(rows, id / NG) * Hkv + g) * NG + id % NG;
+                    ks[i] = __ldg(static_cast<const uint16_t*>(c.ks) + at);
+                    kb[i] = __ldg(static_cast<const uint16_t*>(c.kb) + at);
+                }
+            }
+        };
+        auto load_v = [&](uint32_t rows) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t r = __shfl_sync(0xffffffffu, rows, 16 * mt + 8 * h);
+                    // (the pair's rows follow one another: one page)
+                    const char* at = static_cast<const char*>(c.v) +
+                                     static_cast<size_t>(r == ~0u ? 0u : r + 2 * c4) * row_bytes + g * RB +
+                                     r8 * (RB / 8);
+                    ldw(at, vw[mt][2 * h]);
+                    ldw(at + row_bytes, vw[mt][2 * h + 1]);
+                }
+            if constexpr (BITS != 16) {
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    const int id = 32 * i + lane;
+                    const size_t at = (row_at(rows, id / NG) * Hkv + g) * NG + id % NG;
+                    vs[i] = __ldg(static_cast<const uint16_t*>(c.vs) + at);
+                    vb[i] = __ldg(static_cast<const uint16_t*>(c.vb) + at);
+                }
+            }
+        };
+        int pid = page_id(t0);
 
         // Queries: lane (row r8 of the n-tile, quarter c4) holds its quarter's dims in the
         // order the key words unpack to.
@@ -142,6 +200,11 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
             }
         }
 
+        uint32_t rows = row_id(t0, pid);
+        load_k(rows);
+        load_v(rows);
+        pid = page_id(t0 + 1);
+
         float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -151,113 +214,64 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
             l[nt][0] = l[nt][1] = 0.f;
         }
 
-        // Sixteen keys per warp and step. Eight keys share a page: the two page ids of a
-        // step are loaded a step before its rows, the rows a step before their use (16-bit
-        // rows, which would not fit registers twice, K after S and V after P V).
-        const int te = w.tile_end(a);
-        auto pages = [&](int tile, int (&pid)[2]) {
+        for (int tile = t0; tile < te; ++tile) {
+            const int k0 = tile * KT + warp * 32;
+            // the keys of the 32 that are there, a bit each
+            const uint32_t there = __ballot_sync(0xffffffffu, rows != ~0u);
+            const bool clean = there == ~0u;
+            float sc[NT][2][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int key = tile * KT + warp * 16 + 8 * h;
-                pid[h] = key < kend ? __ldg(bt + (key >> page_shift)) : -1;
-            }
-        };
-        // rows of the pool the two eights begin at; which of them are there, a bit each
-        auto rows = [&](int tile, const int (&pid)[2], uint32_t (&row)[2]) -> uint32_t {
-            uint32_t ok = 0;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const bool good = pid[h] >= 0 && pid[h] < c.pages;
-                const uint32_t in = static_cast<uint32_t>(tile * KT + warp * 16 + 8 * h) & (c.page - 1);
-                ok |= good ? 1u << h : 0u;
-                row[h] = good ? (static_cast<uint32_t>(pid[h]) << page_shift) + in : 0u;  // (page 0: in bounds)
-            }
-            return ok;
-        };
-        auto load_k = [&](Raw<HD, BITS>& x, const uint32_t (&row)[2]) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                ldw(static_cast<const char*>(c.k) + static_cast<size_t>(row[h] + r8) * row_bytes + g * RB +
-                        c4 * (RB / 4),
-                    x.k[h]);
-        };
-        auto load_v = [&](Raw<HD, BITS>& x, const uint32_t (&row)[2]) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const char* at = static_cast<const char*>(c.v) +
-                                 static_cast<size_t>(row[h] + 2 * c4) * row_bytes + g * RB + r8 * (RB / 8);
-                ldw(at, x.v[2 * h]);
-                ldw(at + row_bytes, x.v[2 * h + 1]);
-            }
-            if constexpr (BITS != 16) {
-                const size_t token = row[lane >> 3 & 1] + (lane & 7);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (i == 1 && ng < 4) break;
-                    const size_t at = (token * Hkv + g) * ng + min(lane >> 4, ng - 1) + 2 * i;
-                    x.ks[i] = __ldg(static_cast<const uint16_t*>(c.ks) + at) |
-                              static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(c.kb) + at)) << 16;
-                    x.vs[i] = __ldg(static_cast<const uint16_t*>(c.vs) + at) |
-                              static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(c.vb) + at)) << 16;
-                }
-            }
-        };
-        // scale | bias of (key, this lane's group) from the lane that loaded it
-        auto sb_of = [&](const uint32_t (&x)[2], int key, int group) -> uint32_t {
-            const int from = key + 16 * (group & 1);
-            uint32_t r = __shfl_sync(0xffffffffu, x[0], from);
-            if (ng == 4) {
-                const uint32_t hi = __shfl_sync(0xffffffffu, x[1], from);
-                r = group & 2 ? hi : r;
-            }
-            return r;
-        };
-
-        auto tile_of = [&](int tile, Raw<HD, BITS>& x, uint32_t ok, auto after_s, auto after_pv) {
-            const int k0 = tile * KT + warp * 16;
-            const bool clean = k0 + 16 <= kend && ok == 3u;
-            float sc[NT][4];
-            {
+            for (int mt = 0; mt < 2; ++mt) {
                 uint32_t s2[2] = {0u, 0u}, b2[2] = {0u, 0u};
                 if constexpr (BITS != 16) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t sb = sb_of(x.ks, r8 + 8 * h, kg);
+                        // (the set that holds the id: a constant for each number of groups)
+                        const int set = NG == 1 ? 0 : NG == 2 ? mt : 2 * mt + h;
+                        const int id = (16 * mt + 8 * h + r8) * NG + kg;
+                        const uint32_t sb = __shfl_sync(
+                            0xffffffffu, ks[set] | static_cast<uint32_t>(kb[set]) << 16, id & 31);
                         s2[h] = pk_splat(sb);
                         b2[h] = prmt(sb, 0u, 0x3232u);
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < MT; ++j) {
-                    const uint32_t a0 = row_pair<T, BITS>(x.k[0], 2 * j, s2[0], b2[0]);
-                    const uint32_t a1 = row_pair<T, BITS>(x.k[1], 2 * j, s2[1], b2[1]);
-                    const uint32_t a2 = row_pair<T, BITS>(x.k[0], 2 * j + 1, s2[0], b2[0]);
-                    const uint32_t a3 = row_pair<T, BITS>(x.k[1], 2 * j + 1, s2[1], b2[1]);
+                    const uint32_t a0 = row_pair<T, BITS>(kw[mt][0], 2 * j, s2[0], b2[0]);
+                    const uint32_t a1 = row_pair<T, BITS>(kw[mt][1], 2 * j, s2[1], b2[1]);
+                    const uint32_t a2 = row_pair<T, BITS>(kw[mt][0], 2 * j + 1, s2[0], b2[0]);
+                    const uint32_t a3 = row_pair<T, BITS>(kw[mt][1], 2 * j + 1, s2[1], b2[1]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        if (j == 0) mma16816z<T>(sc[nt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
-                        else mma16816<T>(sc[nt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
+                        if (j == 0) mma16816z<T>(sc[nt][mt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
+                        else mma16816<T>(sc[nt][mt], a0, a1, a2, a3, bq[nt][j][0], bq[nt][j][1]);
                     }
                 }
             }
-            after_s();
-            const bool plain = clean && k0 + 16 <= full;
+            // the next tile's keys come in from here on
+            const uint32_t next = row_id(tile + 1, pid);
+            if (tile + 1 < te) load_k(next);
+            pid = page_id(tile + 2);
+
+            const bool plain = clean && k0 + 32 <= full;
             float grow = -INFINITY;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float y = sc[nt][e] * p.scale_log2;
-                    if (!plain) {
-                        const int key = k0 + r8 + 8 * (e >> 1), j = key - base;
-                        const bool see = key < kend && (ok >> (e >> 1) & 1u) &&
-                                         (j < 0 || (a.mask ? j < 64 && (vis[nt][e & 1] >> (j & 63) & 1)
-                                                           : j <= qpos[nt][e & 1]));
-                        y = see ? y : -INFINITY;
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float y = sc[nt][mt][e] * p.scale_log2;
+                        if (!plain) {
+                            const int x = 16 * mt + 8 * (e >> 1) + r8, j = k0 + x - base;
+                            const bool see = (there >> x & 1u) &&
+                                             (j < 0 || (a.mask ? j < 64 && (vis[nt][e & 1] >> (j & 63) & 1)
+                                                               : j <= qpos[nt][e & 1]));
+                            y = see ? y : -INFINITY;
+                        }
+                        sc[nt][mt][e] = y;
+                        grow = fmaxf(grow, y - m[nt][e & 1]);
                     }
-                    sc[nt][e] = y;
-                    grow = fmaxf(grow, y - m[nt][e & 1]);
-                }
             // The reference of the exponentials follows the running maximum only when a
             // score passes it by 2^8: the probabilities then reach 256, the sums lose nothing.
             if (__any_sync(0xffffffffu, grow > 8.f)) {
@@ -265,7 +279,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(sc[nt][e], sc[nt][e + 2]);
+                        float mx = fmaxf(fmaxf(sc[nt][0][e], sc[nt][0][e + 2]),
+                                         fmaxf(sc[nt][1][e], sc[nt][1][e + 2]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -280,100 +295,63 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
                         }
                     }
             }
-            uint32_t pb[NT][2];
+            uint32_t pb[NT][2][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float pr[4];
+                const float mr[2] = {m[nt][0] == -INFINITY ? 0.f : m[nt][0],
+                                     m[nt][1] == -INFINITY ? 0.f : m[nt][1]};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float mr = m[nt][e & 1];
-                    pr[e] = ex2(sc[nt][e] - (mr == -INFINITY ? 0.f : mr));
-                    l[nt][e & 1] += pr[e];
+                for (int mt = 0; mt < 2; ++mt) {
+                    float pr[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        pr[e] = ex2(sc[nt][mt][e] - mr[e & 1]);
+                        l[nt][e & 1] += pr[e];
+                    }
+                    pb[nt][mt][0] = transpose8x8(pk_round<T>(pr[0], pr[1]));
+                    pb[nt][mt][1] = transpose8x8(pk_round<T>(pr[2], pr[3]));
                 }
-                pb[nt][0] = transpose8x8(pk_round<T>(pr[0], pr[1]));
-                pb[nt][1] = transpose8x8(pk_round<T>(pr[2], pr[3]));
             }
-            uint32_t s2[2] = {0u, 0u}, b2[2] = {0u, 0u};  // of value rows 2 c4, 2 c4 + 1; eight on
-            // values of keys that are not there multiply zeros: make them zeros
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t keep = 0xffffffffu;
-                if (!clean) {
-                    const int k = k0 + 8 * h + 2 * c4;
-                    const bool there = ok >> h & 1u;
-                    keep = (there && k < kend ? 0xffffu : 0u) | (there && k + 1 < kend ? 0xffff0000u : 0u);
-                }
-                if constexpr (BITS == 16) {
-                    if (!clean) {
+            for (int mt = 0; mt < 2; ++mt) {
+                uint32_t s2[2] = {0u, 0u}, b2[2] = {0u, 0u};  // of value rows 2 c4, 2 c4 + 1; eight on
+                // values of keys that are not there multiply zeros: make them zeros
 #pragma unroll
-                        for (int i = 0; i < HD / 16; ++i) {
-                            if (!(keep & 0xffffu)) x.v[2 * h][i] = 0u;
-                            if (!(keep >> 16)) x.v[2 * h + 1][i] = 0u;
+                for (int h = 0; h < 2; ++h) {
+                    const int x = 16 * mt + 8 * h + 2 * c4;
+                    uint32_t keep = 0xffffffffu;
+                    if (!clean)
+                        keep = (there >> x & 1u ? 0xffffu : 0u) | (there >> x & 2u ? 0xffff0000u : 0u);
+                    if constexpr (BITS == 16) {
+                        if (!clean) {
+#pragma unroll
+                            for (int i = 0; i < VW; ++i) {
+                                if (!(keep & 0xffffu)) vw[mt][2 * h][i] = 0u;
+                                if (!(keep >> 16)) vw[mt][2 * h + 1][i] = 0u;
+                            }
                         }
+                    } else {
+                        const int set = NG == 1 ? 0 : NG == 2 ? mt : 2 * mt + h;
+                        const uint32_t sb = vs[set] | static_cast<uint32_t>(vb[set]) << 16;
+                        const uint32_t e0 = __shfl_sync(0xffffffffu, sb, (x * NG + vg) & 31);
+                        const uint32_t e1 = __shfl_sync(0xffffffffu, sb, ((x + 1) * NG + vg) & 31);
+                        s2[h] = prmt(e0, e1, 0x5410u) & keep;
+                        b2[h] = prmt(e0, e1, 0x7632u) & keep;
                     }
-                } else {
-                    const uint32_t e0 = sb_of(x.vs, 8 * h + 2 * c4, vg), e1 = sb_of(x.vs, 8 * h + 2 * c4 + 1, vg);
-                    s2[h] = prmt(e0, e1, 0x5410u) & keep;
-                    b2[h] = prmt(e0, e1, 0x7632u) & keep;
                 }
-            }
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const uint32_t a0 = cross_pair<T, BITS>(x.v[0], x.v[1], i, s2[0], b2[0]);
-                const uint32_t a1 = cross_pair<T, BITS>(x.v[0], x.v[1], MT + i, s2[0], b2[0]);
-                const uint32_t a2 = cross_pair<T, BITS>(x.v[2], x.v[3], i, s2[1], b2[1]);
-                const uint32_t a3 = cross_pair<T, BITS>(x.v[2], x.v[3], MT + i, s2[1], b2[1]);
+                for (int i = 0; i < MT; ++i) {
+                    const uint32_t a0 = cross_pair<T, BITS>(vw[mt][0], vw[mt][1], i, s2[0], b2[0]);
+                    const uint32_t a1 = cross_pair<T, BITS>(vw[mt][0], vw[mt][1], MT + i, s2[0], b2[0]);
+                    const uint32_t a2 = cross_pair<T, BITS>(vw[mt][2], vw[mt][3], i, s2[1], b2[1]);
+                    const uint32_t a3 = cross_pair<T, BITS>(vw[mt][2], vw[mt][3], MT + i, s2[1], b2[1]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-            }
-            after_pv();
-        };
-        auto nothing = [] {};
-
-        if (t0 < te) {
-            int pid[2];
-            uint32_t row[2];
-            pages(t0, pid);
-            uint32_t ok = rows(t0, pid, row);
-            Raw<HD, BITS> x;
-            load_k(x, row);
-            load_v(x, row);
-            pages(t0 + 1, pid);
-            if constexpr (BITS == 16) {
-                for (int tile = t0; tile < te; ++tile) {
-                    uint32_t ok1 = 0;
-                    tile_of(
-                        tile, x, ok,
-                        [&] {
-                            ok1 = rows(tile + 1, pid, row);
-                            if (tile + 1 < te) load_k(x, row);
-                            pages(tile + 2, pid);
-                        },
-                        [&] {
-                            if (tile + 1 < te) load_v(x, row);
-                        });
-                    ok = ok1;
-                }
-            } else {
-                Raw<HD, BITS> y;
-                for (int tile = t0; tile < te; tile += 2) {
-                    const uint32_t ok1 = rows(tile + 1, pid, row);
-                    if (tile + 1 < te) {
-                        load_k(y, row);
-                        load_v(y, row);
-                    }
-                    pages(tile + 2, pid);
-                    tile_of(tile, x, ok, nothing, nothing);
-                    if (tile + 1 >= te) break;
-                    ok = rows(tile + 2, pid, row);
-                    if (tile + 2 < te) {
-                        load_k(x, row);
-                        load_v(x, row);
-                    }
-                    pages(tile + 3, pid);
-                    tile_of(tile + 1, y, ok1, nothing, nothing);
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma16816<T>(o[nt][i], a0, a1, a2, a3, pb[nt][mt][0], pb[nt][mt][1]);
                 }
             }
+            if (tile + 1 < te) load_v(next);
+            rows = next;
         }
 
         // Join the warps: (max, sum, O) of every row through shared memory.
@@ -515,15 +493,22 @@ Plan plan_of(const KvCache& c, const RowsArgs& a) {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-template <typename T, int HD, int BITS>
+template <typename T, int HD, int BITS, int NG>
 const void* rows_fn(int rows) {
-    return rows == 8 ? reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 1>)
-                     : reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, 2>);
+    return rows == 8 ? reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, NG, 1>)
+                     : reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, NG, 2>);
+}
+template <typename T, int HD, int BITS>
+const void* rows_fn(int groups, int rows) {
+    if constexpr (HD == 128) {
+        if (groups == 4) return rows_fn<T, HD, BITS, 4>(rows);
+    }
+    return groups == 2 ? rows_fn<T, HD, BITS, 2>(rows) : rows_fn<T, HD, BITS, 1>(rows);
 }
 template <typename T, int HD>
-const void* rows_fn(int bits, int rows) {
-    return bits == 16 ? rows_fn<T, HD, 16>(rows) : bits == 8 ? rows_fn<T, HD, 8>(rows)
-                                                             : rows_fn<T, HD, 4>(rows);
+const void* rows_fn(int bits, int groups, int rows) {
+    return bits == 16 ? rows_fn<T, HD, 16, 1>(rows) : bits == 8 ? rows_fn<T, HD, 8>(groups, rows)
+                                                                : rows_fn<T, HD, 4>(groups, rows);
 }
 template <typename T, int HD>
 const void* combine_fn(int rows) {
@@ -599,12 +584,14 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& all, void* worksp
         if (pl.tc) {
             e = launch_rows_tc(p, ws, overlap, st);
         } else {
-            const void* f = bf ? (big ? rows_fn<__nv_bfloat16, 128>(c.bits, pl.rows)
-                                      : rows_fn<__nv_bfloat16, 64>(c.bits, pl.rows))
-                               : (big ? rows_fn<__half, 128>(c.bits, pl.rows)
-                                      : rows_fn<__half, 64>(c.bits, pl.rows));
-            static PerDevice cfg[24];
-            e = launch_ex(f, cfg[(type * 3 + (c.bits == 16 ? 0 : c.bits == 8 ? 1 : 2)) * 2 + size],
+            const int ng = c.hd / c.gs;  // 1, 2 or 4
+            const void* f = bf ? (big ? rows_fn<__nv_bfloat16, 128>(c.bits, ng, pl.rows)
+                                      : rows_fn<__nv_bfloat16, 64>(c.bits, ng, pl.rows))
+                               : (big ? rows_fn<__half, 128>(c.bits, ng, pl.rows)
+                                      : rows_fn<__half, 64>(c.bits, ng, pl.rows));
+            static PerDevice cfg[72];
+            e = launch_ex(f,
+                          cfg[((type * 3 + (c.bits == 16 ? 0 : c.bits == 8 ? 1 : 2)) * 3 + ng / 2) * 2 + size],
                           dim3(pl.parts), dim3(ra::THREADS), 0, st, overlap, args);
         }
         if (e != cudaSuccess) return e;
