@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
     w.begin(a, Hkv, un, p.parts, p.group, pref);
     Cut mine = {};
 
+    const float scale = fmaxf(fabsf(p.scale_log2), 0x1p-100f);  // (zero times -inf is no number)
     const int kg = NG == 1 ? 0 : c4 * NG / 4;  // this lane's group of a key row
     const int vg = NG == 1 ? 0 : r8 * NG / 8;  // and of a value row
     const uint32_t row_bytes = static_cast<uint32_t>(Hkv) * RB;  // of a token: its heads' rows
@@ -106,40 +107,37 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
         const int te = w.tile_end(a);
 
         // A warp takes 32 keys of each tile, lane = key of them for the page ids. Eight keys
-        // share a page: eight e of the 32 begins at the row lane 8 e holds; -1: not there.
-        // Page ids are loaded two steps before their use, rows one.
+        // share a page: eight e of the 32 begins at the row lane 8 e holds. Page ids are
+        // loaded two steps before their use, rows one. A row that is not there is read from
+        // the pool's first rows (and not used).
         auto page_id = [&](int tile) -> int {
             const int key = tile * KT + warp * 32 + lane;
             return tile < te && key < kend ? __ldg(bt + (key >> page_shift)) : -1;
         };
         auto row_id = [&](int tile, int pid) -> uint32_t {
-            if (pid < 0 || pid >= c.pages) return ~0u;
-            return (static_cast<uint32_t>(pid) << page_shift) +
-                   (static_cast<uint32_t>(tile * KT + warp * 32 + lane) & (c.page - 1));
-        };
-        // A row that is not there is read from row 0 of the pool (and not used).
-        auto row_at = [&](uint32_t rows, int key) -> size_t {
-            const uint32_t r = __shfl_sync(0xffffffffu, rows, key);
-            return r == ~0u ? 0 : r;
+            const uint32_t in = static_cast<uint32_t>(tile * KT + warp * 32 + lane) & (c.page - 1);
+            return (pid >= 0 && pid < c.pages ? static_cast<uint32_t>(pid) << page_shift : 0u) + in;
         };
         // Words of key rows r8 and r8 + 8 of each sixteen (a quarter of each), of value rows
         // 2 c4, 2 c4 + 1 and eight on (an eighth of each); of 32 keys x NG groups in order,
         // NG to a lane: scales and biases.
         uint32_t kw[2][2][KW], vw[2][4][VW];
         uint16_t ks[NG], kb[NG], vs[NG], vb[NG];
+        const char* k_at = static_cast<const char*>(c.k) + static_cast<size_t>(r8) * row_bytes + g * RB + c4 * (RB / 4);
+        const char* v_at = static_cast<const char*>(c.v) + static_cast<size_t>(2 * c4) * row_bytes + g * RB + r8 * (RB / 8);
         auto load_k = [&](uint32_t rows) {
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    ldw(static_cast<const char*>(c.k) + row_at(rows, 16 * mt + 8 * h + r8) * row_bytes +
-                            g * RB + c4 * (RB / 4),
+                    ldw(k_at + static_cast<size_t>(__shfl_sync(0xffffffffu, rows, 16 * mt + 8 * h)) * row_bytes,
                         kw[mt][h]);
             if constexpr (BITS != 16) {
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     const int id = 32 * i + lane;
-                    const size_t at = (row_at(rows, id / NG) * Hkv + g) * NG + id % NG;
+                    const size_t at = static_cast<size_t>(__shfl_sync(0xffffffffu, rows, id / NG)) * (Hkv * NG) +
+                                      (g * NG + id % NG);
                     ks[i] = __ldg(static_cast<const uint16_t*>(c.ks) + at);
                     kb[i] = __ldg(static_cast<const uint16_t*>(c.kb) + at);
                 }
@@ -150,11 +148,9 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t r = __shfl_sync(0xffffffffu, rows, 16 * mt + 8 * h);
                     // (the pair's rows follow one another: one page)
-                    const char* at = static_cast<const char*>(c.v) +
-                                     static_cast<size_t>(r == ~0u ? 0u : r + 2 * c4) * row_bytes + g * RB +
-                                     r8 * (RB / 8);
+                    const char* at = v_at +
+                        static_cast<size_t>(__shfl_sync(0xffffffffu, rows, 16 * mt + 8 * h)) * row_bytes;
                     ldw(at, vw[mt][2 * h]);
                     ldw(at + row_bytes, vw[mt][2 * h + 1]);
                 }
@@ -162,7 +158,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     const int id = 32 * i + lane;
-                    const size_t at = (row_at(rows, id / NG) * Hkv + g) * NG + id % NG;
+                    const size_t at = static_cast<size_t>(__shfl_sync(0xffffffffu, rows, id / NG)) * (Hkv * NG) +
+                                      (g * NG + id % NG);
                     vs[i] = __ldg(static_cast<const uint16_t*>(c.vs) + at);
                     vb[i] = __ldg(static_cast<const uint16_t*>(c.vb) + at);
                 }
@@ -172,6 +169,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
 
         // Queries: lane (row r8 of the n-tile, quarter c4) holds its quarter's dims in the
         // order the key words unpack to.
+        const uint32_t sign = p.scale_log2 < 0.f ? 0x80008000u : 0u;  // (the scale's goes into them)
         uint32_t bq[NT][MT][2];
         int qpos[NT][2];                // column 2 c4 + e: its index among the new tokens
         unsigned long long vis[NT][2];  // and its ancestors
@@ -189,7 +187,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
             for (int i = 0; i < HD / 8; ++i) {
                 const int da = pair_dim<BITS>(i, 0), db = pair_dim<BITS>(i, 1);
                 bq[nt][i / 2][i % 2] =
-                    prmt(qw[da / 2], qw[db / 2], (da % 2 ? 0x32u : 0x10u) | (db % 2 ? 0x7600u : 0x5400u));
+                    prmt(qw[da / 2], qw[db / 2], (da % 2 ? 0x32u : 0x10u) | (db % 2 ? 0x7600u : 0x5400u)) ^
+                    sign;
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -201,6 +200,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
         }
 
         uint32_t rows = row_id(t0, pid);
+        bool mine_there = pid >= 0 && pid < c.pages;
         load_k(rows);
         load_v(rows);
         pid = page_id(t0 + 1);
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
         for (int tile = t0; tile < te; ++tile) {
             const int k0 = tile * KT + warp * 32;
             // the keys of the 32 that are there, a bit each
-            const uint32_t there = __ballot_sync(0xffffffffu, rows != ~0u);
+            const uint32_t there = __ballot_sync(0xffffffffu, mine_there);
             const bool clean = there == ~0u;
             float sc[NT][2][4];
 #pragma unroll
@@ -250,37 +250,42 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
             }
             // the next tile's keys come in from here on
             const uint32_t next = row_id(tile + 1, pid);
+            mine_there = pid >= 0 && pid < c.pages;
             if (tile + 1 < te) load_k(next);
             pid = page_id(tile + 2);
 
-            const bool plain = clean && k0 + 32 <= full;
-            float grow = -INFINITY;
+            if (!clean || k0 + 32 > full) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
+                    for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float y = sc[nt][mt][e] * p.scale_log2;
-                        if (!plain) {
+                        for (int e = 0; e < 4; ++e) {
                             const int x = 16 * mt + 8 * (e >> 1) + r8, j = k0 + x - base;
                             const bool see = (there >> x & 1u) &&
                                              (j < 0 || (a.mask ? j < 64 && (vis[nt][e & 1] >> (j & 63) & 1)
                                                                : j <= qpos[nt][e & 1]));
-                            y = see ? y : -INFINITY;
+                            sc[nt][mt][e] = see ? sc[nt][mt][e] : -INFINITY;
                         }
-                        sc[nt][mt][e] = y;
-                        grow = fmaxf(grow, y - m[nt][e & 1]);
-                    }
+            }
+            float top[NT][2];
+            bool grow = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    top[nt][e] = fmaxf(fmaxf(sc[nt][0][e], sc[nt][0][e + 2]),
+                                       fmaxf(sc[nt][1][e], sc[nt][1][e + 2])) * scale;
+                    grow |= top[nt][e] > m[nt][e] + 8.f;
+                }
             // The reference of the exponentials follows the running maximum only when a
             // score passes it by 2^8: the probabilities then reach 256, the sums lose nothing.
-            if (__any_sync(0xffffffffu, grow > 8.f)) {
+            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(fmaxf(sc[nt][0][e], sc[nt][0][e + 2]),
-                                         fmaxf(sc[nt][1][e], sc[nt][1][e + 2]));
+                        float mx = top[nt][e];
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
                     float pr[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        pr[e] = ex2(sc[nt][mt][e] - mr[e & 1]);
+                        pr[e] = ex2(fmaf(sc[nt][mt][e], scale, -mr[e & 1]));
                         l[nt][e & 1] += pr[e];
                     }
                     pb[nt][mt][0] = transpose8x8(pk_round<T>(pr[0], pr[1]));

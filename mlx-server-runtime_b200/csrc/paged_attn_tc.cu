@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     extern __shared__ uint8_t rt_smem_raw[];
     __shared__ int pref[SCAN + 1];
     __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], pv_done[2], p_full[2], q_full,
-        q_free, v_land, drained;
+        q_first, q_free, v_land, drained;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_abort;
     uint8_t* smem = rt_smem_raw + ((1024u - (smem_u32(rt_smem_raw) & 1023u)) & 1023u);
@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             mbar_init(smem_u32(pv_done + i), 1);
         }
         mbar_init(smem_u32(&q_full), 1);
+        mbar_init(smem_u32(&q_first), 4);
         mbar_init(smem_u32(&q_free), 1);
         mbar_init(smem_u32(&v_land), 1);
         mbar_init(smem_u32(&drained), 1);
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     w.begin(a, Hkv, un, p.parts, p.group, pref);
 
     // Tile j of the CTA's run uses buffer j & 1 of K, V, S and P, and that buffer's barriers'
-    // phase j >> 1; item i the queries' barriers' phase i. No role is ever two phases behind
+    // phase j >> 1; item i + 1 the queries' barriers' phase i. No role is ever two phases behind
     // another: each buffer's next use waits for its last.
     auto wait_at = [&](uint64_t* bar, uint32_t parity) -> bool {
         if (mbar_try_wait(smem_u32(bar), parity & 1)) return true;
@@ -171,6 +172,29 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             te = max(te, 1);  // (an item without keys: step over it)
         }
         return false;
+    };
+
+    // The segment's queries to shared memory by thread t of n, whole warps of them.
+    auto queries = [&](int t, int n) {
+        constexpr int QL = HD / 8;  // lanes of a row
+        const int inv = 65536 / G + 1;  // x / G = x * inv >> 16 for x < 136
+        const int R = w.s.n * G, n0 = w.rr0 / G, h0 = w.rr0 - n0 * G, ch = t % QL;
+        const T* q = static_cast<const T*>(a.q) +
+                     (static_cast<size_t>(w.s.row0 + n0) * a.Hq + w.g * G) * HD + ch * 8;
+#pragma unroll 8
+        for (int r = t / QL; r < ROWS; r += n / QL) {
+            const int x = h0 + r, dn = x * inv >> 16;
+            const bool in = w.rr0 + r < R;
+            // rows of 128 bytes, sixteen-byte chunks swizzled, a half after the other
+            cp_async16(qs + (ch / 8) * (ROWS * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4),
+                       in ? q + (static_cast<size_t>(dn) * a.Hq + x - dn * G) * HD
+                          : static_cast<const T*>(a.q),
+                       in ? 16 : 0);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        fence_async_smem();
+        __syncwarp();
     };
 
     if (warp == WARP_K || warp == WARP_V) {
@@ -236,30 +260,12 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         }
     } else if (warp > WARP_V) {
         // ------------------------------ queries --------------------------------------
-        constexpr int QL = HD / 8, RPI = 32 / QL;  // lanes of a row, rows at once
-        const int inv = 65536 / G + 1;             // t / G = t * inv >> 16 for t < 136
         uint32_t item = 0;
         for (; w.next(a); w.advance()) {
             if (w.tile_end(a) <= w.t0) continue;
-            if (item > 0 && !wait_at(&q_free, item - 1)) break;  // the last S of the item before
-            ++item;
-            const int R = w.s.n * G, n0 = w.rr0 / G, h0 = w.rr0 - n0 * G, ch = lane % QL;
-            const T* q = static_cast<const T*>(a.q) +
-                         (static_cast<size_t>(w.s.row0 + n0) * a.Hq + w.g * G) * HD + ch * 8;
-#pragma unroll 8
-            for (int r = lane / QL; r < ROWS; r += RPI) {
-                const int t = h0 + r, dn = t * inv >> 16;
-                const bool in = w.rr0 + r < R;
-                // rows of 128 bytes, sixteen-byte chunks swizzled, a half after the other
-                cp_async16(qs + (ch / 8) * (ROWS * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4),
-                           in ? q + (static_cast<size_t>(dn) * a.Hq + t - dn * G) * HD
-                              : static_cast<const T*>(a.q),
-                           in ? 16 : 0);
-            }
-            cp_async_commit();
-            cp_async_wait<0>();
-            fence_async_smem();
-            __syncwarp();
+            if (item++ == 0) continue;  // (the first item's come from the softmax warps)
+            if (!wait_at(&q_free, item - 2)) break;  // the last S of the item before
+            queries(lane, 32);
             if (lane == 0) mbar_arrive(smem_u32(&q_full));
         }
     } else if (warp == WARP_MMA) {
@@ -287,7 +293,9 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             const bool begin = tile == w.t0;
             const uint32_t bit = 1u << (ns & 31), buf = ns & 1;
             begins = begin ? begins | bit : begins & ~bit;
-            if ((begin && !spin(&q_full, nq++)) || !spin(k_full + buf, ns >> 1)) {
+            const bool met = !begin || (nq == 0 ? spin(&q_first, 0) : spin(&q_full, nq - 1));
+            nq += begin ? 1 : 0;
+            if (!met || !spin(k_full + buf, ns >> 1)) {
                 ok = false;
                 return;
             }
@@ -333,6 +341,10 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         for (; ok && w.next(a); w.advance()) {
             const Seq& s = w.s;
             const int kend = w.kend(a), te = w.tile_end(a), base = w.base(), R = s.n * G;
+            if (it == 0 && te > w.t0) {  // the run's first queries: nothing else to do yet
+                queries(tid, 128);
+                if (lane == 0) mbar_arrive(smem_u32(&q_first));
+            }
             const int rr = w.rr0 + row;
             const bool active = rr < R, some = w.rr0 + warp * 32 < R;  // this row; any of the warp's
             const int full = min(max(base, 0), kend);  // keys every row sees
@@ -491,55 +503,59 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
 
 // The values of every sequence's keys, from the first to the end of its last tile (zeros
 // behind the last key and for pages outside the pool): block (tile of 64 keys, sequence,
-// keys or values), thread = 16 bytes of codes at a time, four of them in flight.
+// keys or values), thread = eight values at a time, so that a warp reads and writes one
+// span, eight of them in flight.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
     kv_expand_kernel(const KvCache c, const RowsArgs a, int rows_per_seq, T* __restrict__ k_out,
                      T* __restrict__ v_out) {
-    constexpr int CPU = 16 / BITS, AHEAD = 4;  // chunks of eight values in 16 bytes
+    constexpr int AHEAD = 8;
     pdl_launch_dependents();
     pdl_wait();
     const bool is_v = blockIdx.z != 0;
     const int b = blockIdx.y, k0 = blockIdx.x * rt::KT;
     const int L = max(0, min(a.kv_lens[b], a.max_kv));
     if (k0 >= L) return;
-    const int upr = c.Hkv * c.hd * BITS / 128, units = rt::KT * upr;  // of 16 bytes, in a row
+    const int cpr = c.Hkv * c.hd / 8, chunks = rt::KT * cpr;  // of eight values, in a row
     const int32_t* bt = a.table + static_cast<size_t>(b) * a.max_blocks;
-    const int page_shift = 31 - __clz(c.page), gpu = 128 / BITS;     // (elements of a unit)
-    const uint4* codes = static_cast<const uint4*>(is_v ? c.v : c.k);
+    const int page_shift = 31 - __clz(c.page), gs_shift = 31 - __clz(c.gs);
+    const uint32_t* codes = static_cast<const uint32_t*>(is_v ? c.v : c.k);
     const uint16_t* sp = static_cast<const uint16_t*>(is_v ? c.vs : c.ks);
     const uint16_t* bp = static_cast<const uint16_t*>(is_v ? c.vb : c.kb);
     uint4* out = reinterpret_cast<uint4*>(is_v ? v_out : k_out) +
-                 (static_cast<size_t>(b) * rows_per_seq + k0) * upr * CPU;
-    for (int i0 = threadIdx.x; i0 < units; i0 += 256 * AHEAD) {
-        uint4 raw[AHEAD];
-        uint32_t s[AHEAD], z[AHEAD];
+                 (static_cast<size_t>(b) * rows_per_seq + k0) * cpr;
+    for (int i0 = threadIdx.x; i0 < chunks; i0 += 256 * AHEAD) {
+        uint32_t raw[AHEAD][BITS / 4];
+        uint16_t s[AHEAD], z[AHEAD];
+        uint32_t there = 0;
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const int i = i0 + j * 256, row = i / upr, key = k0 + row;
-            raw[j] = make_uint4(0u, 0u, 0u, 0u);
-            s[j] = z[j] = 0u;
-            if (i < units && key < L) {
-                const int pid = __ldg(bt + (key >> page_shift));
-                if (pid >= 0 && pid < c.pages) {
-                    const size_t at = ((static_cast<size_t>(pid) << page_shift) + (key & (c.page - 1))) * upr +
-                                      (i - row * upr);
-                    raw[j] = __ldg(codes + at);
-                    const size_t g = at * gpu / c.gs;
-                    s[j] = __ldg(sp + g);
-                    z[j] = __ldg(bp + g);
-                }
+            const int i = i0 + j * 256, row = i / cpr, key = k0 + row;
+            int pid = -1;
+            if (i < chunks && key < L) pid = __ldg(bt + (key >> page_shift));
+            const bool in = pid >= 0 && pid < c.pages;
+            there |= in ? 1u << j : 0u;
+            // (a chunk that is not there is read from the pool's first, and not used)
+            const size_t at = in ? ((static_cast<size_t>(pid) << page_shift) + (key & (c.page - 1))) * cpr +
+                                       (i - row * cpr)
+                                 : 0;
+            if constexpr (BITS == 8) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(codes) + at);
+                raw[j][0] = v.x;
+                raw[j][1] = v.y;
+            } else {
+                raw[j][0] = __ldg(codes + at);
             }
+            s[j] = __ldg(sp + (at * 8 >> gs_shift));
+            z[j] = __ldg(bp + (at * 8 >> gs_shift));
         }
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             const int i = i0 + j * 256;
-            if (i >= units) break;
-            const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-#pragma unroll
-            for (int q = 0; q < CPU; ++q)
-                out[static_cast<size_t>(i) * CPU + q] =
-                    in_order<T, BITS>(w + q * (BITS / 4), pk_splat(s[j]), pk_splat(z[j]));
+            if (i >= chunks) break;
+            uint4 o = make_uint4(0u, 0u, 0u, 0u);
+            if (there >> j & 1u) o = in_order<T, BITS>(raw[j], pk_splat(s[j]), pk_splat(z[j]));
+            out[i] = o;
         }
     }
 }

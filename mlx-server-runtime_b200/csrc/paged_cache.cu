@@ -62,23 +62,28 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
     const int slot = a.slots[t];
     const double pos = static_cast<double>(a.positions[t]);
     const bool keep = slot >= 0 && slot < c.pages * static_cast<long long>(c.page);
+    const int heads = a.Hq + 2 * c.Hkv;
+    const int first = (blockIdx.y * (blockDim.x >> 5) + warp) * a.rounds * HPW + lane / LPH;
+    const T* src = static_cast<const T*>(a.qkv) + t * a.ld;
+    uint2 next[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+    auto fetch = [&](int h) {  // a head's elements, a round before they are used
+        if (h < heads) {
+            next[0] = ld8(src + static_cast<size_t>(h) * HD + e0);
+            next[1] = ld8(src + static_cast<size_t>(h) * HD + HALF + e0);
+        }
+    };
+    fetch(first);
     float cs[4], sn[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const double x = pos * turn[j];
         sincospif(2.0f * static_cast<float>(x - rint(x)), &sn[j], &cs[j]);
     }
-    const int heads = a.Hq + 2 * c.Hkv;
-    const int first = (blockIdx.y * (blockDim.x >> 5) + warp) * a.rounds * HPW + lane / LPH;
-    const T* src = static_cast<const T*>(a.qkv) + t * a.ld;
     for (int r = 0; r < a.rounds; ++r) {
         const int h = first + r * HPW;
         const bool live = h < heads;
-        uint2 lo = make_uint2(0u, 0u), hi = lo;
-        if (live) {
-            lo = ld8(src + static_cast<size_t>(h) * HD + e0);
-            hi = ld8(src + static_cast<size_t>(h) * HD + HALF + e0);
-        }
+        uint2 lo = next[0], hi = next[1];
+        if (r + 1 < a.rounds) fetch(h + HPW);
         float x[4] = {Elem<T>::lo(lo.x), Elem<T>::hi(lo.x), Elem<T>::lo(lo.y), Elem<T>::hi(lo.y)};
         float y[4] = {Elem<T>::lo(hi.x), Elem<T>::hi(hi.x), Elem<T>::lo(hi.y), Elem<T>::hi(hi.y)};
         const bool is_q = h < a.Hq, is_v = h >= a.Hq + c.Hkv;
