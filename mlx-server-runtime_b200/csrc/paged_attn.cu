@@ -433,7 +433,11 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
         float v[AHEAD][DPL];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int k = min(k0 + i * c.step, c.last);
+            const int k = k0 + i * c.step;
+            ml[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int e = 0; e < DPL; ++e) v[i][e] = 0.f;
+            if (k > c.last) continue;
             const size_t at = static_cast<size_t>(k == first ? c.slot : 2 * k) * ROWS + r;
             ml[i] = __ldcg(&p.part_ml[at]);
             if constexpr (DPL == 4) {
@@ -444,17 +448,22 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
                 v[i][0] = t.x; v[i][1] = t.y;
             }
         }
+        // one maximum for the eight and what went before
+        float Mn = M;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) Mn = fmaxf(Mn, ml[i].x);
+        const float co = M == -INFINITY ? 0.f : ex2(M - Mn);
+        den *= co;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) acc[e] *= co;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            if (k0 + i * c.step > c.last) break;
-            const float Mn = fmaxf(M, ml[i].x);
-            const float co = M == -INFINITY ? 0.f : exp2f(M - Mn);
-            const float cn = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - Mn);
-            den = fmaf(cn, ml[i].y, den * co);
+            const float cn = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - Mn);
+            den = fmaf(cn, ml[i].y, den);
 #pragma unroll
-            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(cn, v[i][e], acc[e] * co);
-            M = Mn;
+            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(cn, v[i][e], acc[e]);
         }
+        M = Mn;
     }
     const float inv = M == -INFINITY ? 0.f : 1.0f / den;
     const int rr = c.rr0 + r;
