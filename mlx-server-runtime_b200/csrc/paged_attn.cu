@@ -410,34 +410,42 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
     if (tid == 0) p.cut[blockIdx.x] = mine;
 }
 
-// Joins the parts of the items that several CTAs took: block (CTA that began one, eight
-// rows), warp = row, lane = HD / 32 dimensions. Parts are taken in order of keys, eight
-// loads ahead.
+// Joins the parts of the items that several CTAs took: block (CTA that began one, a few of
+// its rows), lane = HD / 32 dimensions. Eight rows in 128 are many: a warp to a row. A
+// decode step's eight are few, and a long sequence alone on the GPU has a part on every
+// fourth CTA: two rows to a block, four warps to a row, each a run of the parts. Parts are
+// taken in order of keys, eight loads ahead.
 template <typename T, int HD, int ROWS>
 __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant__ ra::Params p) {
     using namespace ra;
-    constexpr int DPL = HD / 32, AHEAD = 8;
+    constexpr int DPL = HD / 32, AHEAD = 8, S = ROWS == 128 ? 1 : 4, RPB = 8 / S;
+    __shared__ float so[S > 1 ? 8 : 1][HD];
+    __shared__ float2 sml[8];
     pdl_launch_dependents();
     pdl_wait();
     const Cut c = p.cut[blockIdx.x];
     const RowsArgs& a = p.a;
-    const int G = a.Hq / p.c.Hkv, lane = threadIdx.x & 31;
-    const int r = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (r >= c.rows) return;
+    const int G = a.Hq / p.c.Hkv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (static_cast<int>(blockIdx.y) * RPB >= c.rows) return;
+    const int r = blockIdx.y * RPB + warp / S;
+    const bool live = r < c.rows;
     const int first = blockIdx.x;
+    // the warp's run of parts
+    const int n = (c.last - first) / c.step + 1, per = (n + S - 1) / S;
+    const int lo = warp % S * per, hi = live ? min(n, lo + per) : 0;
     float M = -INFINITY, den = 0.f, acc[DPL];
 #pragma unroll
     for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
-    for (int k0 = first; k0 <= c.last; k0 += AHEAD * c.step) {
+    for (int i0 = lo; i0 < hi; i0 += AHEAD) {
         float2 ml[AHEAD];
         float v[AHEAD][DPL];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int k = k0 + i * c.step;
             ml[i] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int e = 0; e < DPL; ++e) v[i][e] = 0.f;
-            if (k > c.last) continue;
+            if (i0 + i >= hi) continue;
+            const int k = first + (i0 + i) * c.step;
             const size_t at = static_cast<size_t>(k == first ? c.slot : 2 * k) * ROWS + r;
             ml[i] = __ldcg(&p.part_ml[at]);
             if constexpr (DPL == 4) {
@@ -465,6 +473,29 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
         }
         M = Mn;
     }
+    if constexpr (S > 1) {  // the row's warps, in order
+        if (lane == 0) sml[warp] = make_float2(M, den);
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) so[warp][lane * DPL + e] = acc[e];
+        __syncthreads();
+        if (warp % S != 0) return;
+        float Mn = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < S; ++i) Mn = fmaxf(Mn, sml[warp + i].x);
+        den = 0.f;
+#pragma unroll
+        for (int e = 0; e < DPL; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const float2 ml = sml[warp + i];
+            const float cn = ml.x == -INFINITY ? 0.f : ex2(ml.x - Mn);
+            den = fmaf(cn, ml.y, den);
+#pragma unroll
+            for (int e = 0; e < DPL; ++e) acc[e] = fmaf(cn, so[warp + i][lane * DPL + e], acc[e]);
+        }
+        M = Mn;
+    }
+    if (!live) return;
     const float inv = M == -INFINITY ? 0.f : 1.0f / den;
     const int rr = c.rr0 + r;
     T* dst = static_cast<T*>(a.out) +
@@ -615,7 +646,7 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& all, void* worksp
                                    : combine_fn<__nv_bfloat16, 64>(pl.rows))
                             : (big ? combine_fn<__half, 128>(pl.rows) : combine_fn<__half, 64>(pl.rows));
         static PerDevice cfgc[12];
-        e = launch_ex(fc, cfgc[type * 3 + size], dim3(pl.parts - 1, pl.rows / 8), dim3(256), 0,
+        e = launch_ex(fc, cfgc[type * 3 + size], dim3(pl.parts - 1, pl.rows == 128 ? 16 : pl.rows / 2), dim3(256), 0,
                       st, true, args);
         if (e != cudaSuccess) return e;
     }

@@ -503,8 +503,8 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
 
 // The values of every sequence's keys, from the first to the end of its last tile (zeros
 // behind the last key and for pages outside the pool): block (tile of 64 keys, sequence,
-// keys or values), thread = eight values at a time, so that a warp reads and writes one
-// span, eight of them in flight.
+// keys or values), thread = (eight values of a row, row), so that a warp reads and writes
+// one span; eight rows in flight.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
     kv_expand_kernel(const KvCache c, const RowsArgs a, int rows_per_seq, T* __restrict__ k_out,
@@ -516,46 +516,47 @@ __global__ void __launch_bounds__(256)
     const int b = blockIdx.y, k0 = blockIdx.x * rt::KT;
     const int L = max(0, min(a.kv_lens[b], a.max_kv));
     if (k0 >= L) return;
-    const int cpr = c.Hkv * c.hd / 8, chunks = rt::KT * cpr;  // of eight values, in a row
+    const uint32_t cpr = c.Hkv * c.hd / 8;                       // chunks of eight values in a row
+    const int page_shift = 31 - __clz(c.page), gs_shift = 28 - __clz(c.gs);  // (of chunks)
+    const uint32_t gpr = cpr >> gs_shift;                        // groups in a row
     const int32_t* bt = a.table + static_cast<size_t>(b) * a.max_blocks;
-    const int page_shift = 31 - __clz(c.page), gs_shift = 31 - __clz(c.gs);
-    const uint32_t* codes = static_cast<const uint32_t*>(is_v ? c.v : c.k);
-    const uint16_t* sp = static_cast<const uint16_t*>(is_v ? c.vs : c.ks);
-    const uint16_t* bp = static_cast<const uint16_t*>(is_v ? c.vb : c.kb);
-    uint4* out = reinterpret_cast<uint4*>(is_v ? v_out : k_out) +
-                 (static_cast<size_t>(b) * rows_per_seq + k0) * cpr;
-    for (int i0 = threadIdx.x; i0 < chunks; i0 += 256 * AHEAD) {
-        uint32_t raw[AHEAD][BITS / 4];
-        uint16_t s[AHEAD], z[AHEAD];
-        uint32_t there = 0;
+    for (uint32_t col = threadIdx.x; col < cpr; col += blockDim.x) {
+        const uint32_t* codes = static_cast<const uint32_t*>(is_v ? c.v : c.k) + col * (BITS / 4);
+        const uint16_t* sp = static_cast<const uint16_t*>(is_v ? c.vs : c.ks) + (col >> gs_shift);
+        const uint16_t* bp = static_cast<const uint16_t*>(is_v ? c.vb : c.kb) + (col >> gs_shift);
+        uint4* out = reinterpret_cast<uint4*>(is_v ? v_out : k_out) +
+                     (static_cast<size_t>(b) * rows_per_seq + k0) * cpr + col;
+        for (uint32_t r0 = threadIdx.y; r0 < rt::KT; r0 += AHEAD * blockDim.y) {
+            uint32_t raw[AHEAD][BITS / 4], there = 0;
+            uint16_t s[AHEAD], z[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const int i = i0 + j * 256, row = i / cpr, key = k0 + row;
-            int pid = -1;
-            if (i < chunks && key < L) pid = __ldg(bt + (key >> page_shift));
-            const bool in = pid >= 0 && pid < c.pages;
-            there |= in ? 1u << j : 0u;
-            // (a chunk that is not there is read from the pool's first, and not used)
-            const size_t at = in ? ((static_cast<size_t>(pid) << page_shift) + (key & (c.page - 1))) * cpr +
-                                       (i - row * cpr)
-                                 : 0;
-            if constexpr (BITS == 8) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(codes) + at);
-                raw[j][0] = v.x;
-                raw[j][1] = v.y;
-            } else {
-                raw[j][0] = __ldg(codes + at);
+            for (int j = 0; j < AHEAD; ++j) {
+                const int r = r0 + j * blockDim.y, key = k0 + r;
+                int pid = -1;
+                if (r < rt::KT && key < L) pid = __ldg(bt + (key >> page_shift));
+                const bool in = pid >= 0 && pid < c.pages;
+                there |= in ? 1u << j : 0u;
+                // (a row that is not there is read from the pool's first, and not used)
+                const uint32_t row = in ? (static_cast<uint32_t>(pid) << page_shift) + (key & (c.page - 1)) : 0u;
+                const uint32_t* at = codes + static_cast<size_t>(row) * (cpr * (BITS / 4));
+                if constexpr (BITS == 8) {
+                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+                    raw[j][0] = v.x;
+                    raw[j][1] = v.y;
+                } else {
+                    raw[j][0] = __ldg(at);
+                }
+                s[j] = __ldg(sp + static_cast<size_t>(row) * gpr);
+                z[j] = __ldg(bp + static_cast<size_t>(row) * gpr);
             }
-            s[j] = __ldg(sp + (at * 8 >> gs_shift));
-            z[j] = __ldg(bp + (at * 8 >> gs_shift));
-        }
 #pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const int i = i0 + j * 256;
-            if (i >= chunks) break;
-            uint4 o = make_uint4(0u, 0u, 0u, 0u);
-            if (there >> j & 1u) o = in_order<T, BITS>(raw[j], pk_splat(s[j]), pk_splat(z[j]));
-            out[i] = o;
+            for (int j = 0; j < AHEAD; ++j) {
+                const uint32_t r = r0 + j * blockDim.y;
+                if (r >= rt::KT) break;
+                uint4 o = make_uint4(0u, 0u, 0u, 0u);
+                if (there >> j & 1u) o = in_order<T, BITS>(raw[j], pk_splat(s[j]), pk_splat(z[j]));
+                out[static_cast<size_t>(r) * cpr] = o;
+            }
         }
     }
 }
@@ -614,6 +615,7 @@ cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStre
         if (rps == 0) rps = rt::KT;
         const size_t each = static_cast<size_t>(p.a.batch) * rps * c.Hkv * c.hd * 2;
         void *ko = expanded, *vo = static_cast<char*>(expanded) + each;
+        const int cpr = c.Hkv * c.hd / 8, x = cpr < 256 ? cpr : 256;
         KvCache cc = c;
         RowsArgs aa = p.a;
         void* args[] = {&cc, &aa, &rps, &ko, &vo};
@@ -623,7 +625,8 @@ cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStre
                                           : reinterpret_cast<const void*>(&kv_expand_kernel<__half, 4>));
         static PerDevice cfg[4];
         const cudaError_t e = launch_ex(f, cfg[(bf ? 0 : 2) + (c.bits == 8 ? 0 : 1)],
-                                        dim3(rps / rt::KT, p.a.batch, 2), dim3(256), 0, st, overlap, args);
+                                        dim3(rps / rt::KT, p.a.batch, 2), dim3(x, 256 / x), 0, st,
+                                        overlap, args);
         if (e != cudaSuccess) return e;
         overlap = true;  // (the attention waits for the whole of it)
         k = ko;
