@@ -90,8 +90,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
 
     zero_tail(a, HD, THREADS);
     const Units un = scan_units<KT>(a, Hkv, G, ROWS, p.group, pref);
-    Walk<KT, ROWS> w;
-    w.begin(a, Hkv, un, p.parts, p.group, pref);
+    Walk<KT> w;
+    w.begin(a, Hkv, ROWS, un, p.parts, p.group, pref);
     Cut mine = {};
 
     const float scale = fmaxf(fabsf(p.scale_log2), 0x1p-100f);  // (zero times -inf is no number)
@@ -509,26 +509,32 @@ __global__ void __launch_bounds__(256) attn_combine_kernel(const __grid_constant
 
 namespace {
 
-// How a call is run: eight rows to a chunk where a decode step's heads fit them, sixteen
-// up to there, and from then on 128 of them as the M rows of tcgen05 products.
+// How a call is run: eight rows to a chunk where a decode step's heads fit them; sixteen
+// of a quantised cache; and from then on up to 128, whole tokens of them, as the M rows of
+// tcgen05 products. (Eight sequences of 4096 keys, seven heads to a kv head: two tokens over
+// 4 bits 23 us with sixteen rows to a chunk and 36 as M rows, whose keys are expanded first;
+// over 16 bits 33 and 26.)
 struct Plan {
     bool tc;
     int rows, kt, parts, group;
+    int chunk;  // rows of a chunk: `rows`, or the whole tokens of them
 };
 Plan plan_of(const KvCache& c, const RowsArgs& a) {
-    const long long r = static_cast<long long>(a.max_q) * (a.Hq / c.Hkv);
+    const int G = a.Hq / c.Hkv;
+    const long long r = static_cast<long long>(a.max_q) * G;
     Plan p;
-    p.tc = r > 16;
+    p.tc = r > (c.bits == 16 ? 8 : 16);
     p.rows = p.tc ? 128 : r > 8 ? 16 : 8;
+    p.chunk = p.tc ? 128 / G * G : p.rows;
     p.kt = p.tc ? kRowsTcKeys : ra::KT;
     // CTAs the units are shared out to: what the GPU holds at once, at most one per unit
     const long long most = 148LL * (p.tc ? 2 : ra::resident(c.hd, c.bits, p.rows / 8));
     const long long tiles = (a.max_kv + p.kt - 1) / p.kt;
-    long long units = (r + p.rows - 1) / p.rows * (tiles > 0 ? tiles : 1) * c.Hkv;
+    long long units = (r + p.chunk - 1) / p.chunk * (tiles > 0 ? tiles : 1) * c.Hkv;
     units = units < most ? units * a.batch : most;
     p.parts = static_cast<int>(units < 1 ? 1 : units < most ? units : most);
     // up to eight chunks go side by side
-    const int chunks = static_cast<int>((r + p.rows - 1) / p.rows);
+    const int chunks = static_cast<int>((r + p.chunk - 1) / p.chunk);
     p.group = p.tc && chunks >= 2 && chunks <= 8 ? chunks : 1;
     if (p.group > 1) p.parts = (p.parts + p.group - 1) / p.group * p.group > most
                                    ? static_cast<int>(most / p.group * p.group)
@@ -540,8 +546,10 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 template <typename T, int HD, int BITS, int NG>
 const void* rows_fn(int rows) {
-    return rows == 8 ? reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, NG, 1>)
-                     : reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, NG, 2>);
+    if constexpr (BITS != 16) {
+        if (rows == 16) return reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, NG, 2>);
+    }
+    return reinterpret_cast<const void*>(&attn_rows_kernel<T, HD, BITS, NG, 1>);
 }
 template <typename T, int HD, int BITS>
 const void* rows_fn(int groups, int rows) {
@@ -567,7 +575,7 @@ const void* combine_fn(int rows) {
 bool attn_rows_countable(const KvCache& c, const RowsArgs& a) {
     const Plan pl = plan_of(c, a);
     const long long r = static_cast<long long>(a.max_q) * (a.Hq / c.Hkv);
-    const double units = static_cast<double>((r + pl.rows - 1) / pl.rows) * c.Hkv * a.batch *
+    const double units = static_cast<double>((r + pl.chunk - 1) / pl.chunk) * c.Hkv * a.batch *
                          (a.max_kv / pl.kt + 1);
     return units < 2147483647.0;
 }

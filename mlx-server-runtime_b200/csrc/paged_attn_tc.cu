@@ -17,8 +17,10 @@
 // one ends, and P V runs under the next softmax. Warps 0-3 hold a tensor-memory lane quarter
 // each and do the softmax and the epilogue; warp 4 brings keys in by TMA and warp 6 values, a
 // box to a page and 64 dims (one warp for both takes 2100 cycles a tile of 16-key pages,
-// longer than the softmax); warp 5 issues the products; warp 7 brings the queries of the
-// next item. Two CTAs share an SM (96 KB of shared memory and 256 columns each).
+// longer than the softmax); warp 5 issues the products. A chunk is whole tokens, 128 / G of
+// them, so that its queries are one box too (64 dims, G heads, the tokens): loaded by a
+// warp's lanes they took 5000 cycles of every item. Two CTAs share an SM (96 KB of shared
+// memory and 256 columns each).
 // Work is shared out as in rows_units.cuh. Every wait is bounded: on a timeout the CTA
 // records an error, its roles stop, what is in flight is waited for, tensor memory is
 // freed and the kernel returns.
@@ -39,7 +41,7 @@ __device__ int g_rows_tc_error;  // 0, or the first error code a kernel recorded
 
 namespace rt {
 constexpr int ROWS = 128, KT = kRowsTcKeys, THREADS = kRowsTcThreads;
-constexpr int WARP_K = 4, WARP_MMA = 5, WARP_V = 6;  // and 7: queries
+constexpr int WARP_K = 4, WARP_MMA = 5, WARP_V = 6;
 constexpr uint32_t kCols = 256;   // tensor memory: S (and P) from 0 and 64, O from 128
 constexpr uint32_t kOCol = 128;
 constexpr uint32_t kParkNs = 2000, kParkLimit = 1u << 20;  // ~2 s
@@ -85,7 +87,8 @@ struct RowSource {
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(rt::THREADS, 2)
-    attn_rows_tc_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+    attn_rows_tc_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
+                        const __grid_constant__ CUtensorMap tv,
                         const __grid_constant__ ra::Params p, const RowSource src) {
     using namespace rt;
     using namespace ra;
@@ -98,7 +101,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     extern __shared__ uint8_t rt_smem_raw[];
     __shared__ int pref[SCAN + 1];
     __shared__ __align__(8) uint64_t k_full[2], v_full[2], s_full[2], pv_done[2], p_full[2], q_full,
-        q_first, q_free, v_land, drained;
+        q_free, v_land, drained;
     __shared__ uint32_t tmem_slot;
     __shared__ volatile int s_abort;
     uint8_t* smem = rt_smem_raw + ((1024u - (smem_u32(rt_smem_raw) & 1023u)) & 1023u);
@@ -120,31 +123,33 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             mbar_init(smem_u32(pv_done + i), 1);
         }
         mbar_init(smem_u32(&q_full), 1);
-        mbar_init(smem_u32(&q_first), 4);
         mbar_init(smem_u32(&q_free), 1);
         mbar_init(smem_u32(&v_land), 1);
         mbar_init(smem_u32(&drained), 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
-    if (warp == WARP_K && lane == 0) tma_prefetch_map(&tk);
+    if (warp == WARP_K && lane == 0) {
+        tma_prefetch_map(&tq);
+        tma_prefetch_map(&tk);
+    }
     if (warp == WARP_V && lane == 0) tma_prefetch_map(&tv);
     pdl_wait();
     const RowsArgs& a = p.a;
     const KvCache& c = p.c;
-    const int Hkv = c.Hkv, G = a.Hq / Hkv;
+    const int Hkv = c.Hkv, G = a.Hq / Hkv, chunk = ROWS / G * G;
     zero_tail(a, HD, THREADS);
-    const Units un = scan_units<KT>(a, Hkv, G, ROWS, p.group, pref);
+    const Units un = scan_units<KT>(a, Hkv, G, chunk, p.group, pref);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int page_shift = 31 - __clz(c.page);
-    Walk<KT, ROWS> w;
-    w.begin(a, Hkv, un, p.parts, p.group, pref);
+    Walk<KT> w;
+    w.begin(a, Hkv, chunk, un, p.parts, p.group, pref);
 
     // Tile j of the CTA's run uses buffer j & 1 of K, V, S and P, and that buffer's barriers'
-    // phase j >> 1; item i + 1 the queries' barriers' phase i. No role is ever two phases behind
+    // phase j >> 1; item i the queries' barriers' phase i. No role is ever two phases behind
     // another: each buffer's next use waits for its last.
     auto wait_at = [&](uint64_t* bar, uint32_t parity) -> bool {
         if (mbar_try_wait(smem_u32(bar), parity & 1)) return true;
@@ -174,29 +179,6 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         return false;
     };
 
-    // The segment's queries to shared memory by thread t of n, whole warps of them.
-    auto queries = [&](int t, int n) {
-        constexpr int QL = HD / 8;  // lanes of a row
-        const int inv = 65536 / G + 1;  // x / G = x * inv >> 16 for x < 136
-        const int R = w.s.n * G, n0 = w.rr0 / G, h0 = w.rr0 - n0 * G, ch = t % QL;
-        const T* q = static_cast<const T*>(a.q) +
-                     (static_cast<size_t>(w.s.row0 + n0) * a.Hq + w.g * G) * HD + ch * 8;
-#pragma unroll 8
-        for (int r = t / QL; r < ROWS; r += n / QL) {
-            const int x = h0 + r, dn = x * inv >> 16;
-            const bool in = w.rr0 + r < R;
-            // rows of 128 bytes, sixteen-byte chunks swizzled, a half after the other
-            cp_async16(qs + (ch / 8) * (ROWS * 128) + r * 128 + (((ch % 8) ^ (r & 7)) << 4),
-                       in ? q + (static_cast<size_t>(dn) * a.Hq + x - dn * G) * HD
-                          : static_cast<const T*>(a.q),
-                       in ? 16 : 0);
-        }
-        cp_async_commit();
-        cp_async_wait<0>();
-        fence_async_smem();
-        __syncwarp();
-    };
-
     if (warp == WARP_K || warp == WARP_V) {
         // ------------------------------ keys, values ---------------------------------
         // lane = (box of the tile, 64-dim half); a box that is not there is read from behind
@@ -214,11 +196,20 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             if (src.rows_per_seq) return w.b * src.rows_per_seq + key;
             return __ldg(a.table + static_cast<size_t>(w.b) * a.max_blocks + (key >> page_shift));
         };
-        uint32_t j = 0, lands = 0;
+        uint32_t j = 0, lands = 0, items = 0;
         bool more = step();
         int page = more ? page_of() : -1;
         for (; more; ++j) {
             const int g = w.g, left = kend - tile * KT;  // keys of the tile
+            if (!is_v && tile == w.t0) {  // the item's queries, once the last S of the one before is done
+                if (items > 0 && !wait_at(&q_free, items - 1)) break;
+                ++items;
+                if (lane == 0) mbar_arrive_expect_tx(smem_u32(&q_full), chunk * HD * 2);
+                __syncwarp();
+                if (lane < HALVES)
+                    tma_load_3d(smem_u32(qs) + lane * (ROWS * 128), &tq, smem_u32(&q_full), lane * 64, g * G,
+                                w.s.row0 + w.rr0 / G);
+            }
             const int row = page < 0 ? src.rows
                             : src.rows_per_seq ? page
                             : page < c.pages   ? page << page_shift
@@ -257,16 +248,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             for (uint32_t i = j > 1 ? j - 2 : 0; i < j; ++i)
                 mbar_wait_bounded(smem_u32(full + (i & 1)), (i >> 1) & 1, kSpinLimit);
             if (lands) mbar_wait_bounded(smem_u32(&v_land), (lands - 1) & 1, kSpinLimit);
-        }
-    } else if (warp > WARP_V) {
-        // ------------------------------ queries --------------------------------------
-        uint32_t item = 0;
-        for (; w.next(a); w.advance()) {
-            if (w.tile_end(a) <= w.t0) continue;
-            if (item++ == 0) continue;  // (the first item's come from the softmax warps)
-            if (!wait_at(&q_free, item - 2)) break;  // the last S of the item before
-            queries(lane, 32);
-            if (lane == 0) mbar_arrive(smem_u32(&q_full));
+            if (items) mbar_wait_bounded(smem_u32(&q_full), (items - 1) & 1, kSpinLimit);
         }
     } else if (warp == WARP_MMA) {
         // ------------------------------ products -------------------------------------
@@ -293,9 +275,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             const bool begin = tile == w.t0;
             const uint32_t bit = 1u << (ns & 31), buf = ns & 1;
             begins = begin ? begins | bit : begins & ~bit;
-            const bool met = !begin || (nq == 0 ? spin(&q_first, 0) : spin(&q_full, nq - 1));
-            nq += begin ? 1 : 0;
-            if (!met || !spin(k_full + buf, ns >> 1)) {
+            if ((begin && !spin(&q_full, nq++)) || !spin(k_full + buf, ns >> 1)) {
                 ok = false;
                 return;
             }
@@ -341,12 +321,9 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         for (; ok && w.next(a); w.advance()) {
             const Seq& s = w.s;
             const int kend = w.kend(a), te = w.tile_end(a), base = w.base(), R = s.n * G;
-            if (it == 0 && te > w.t0) {  // the run's first queries: nothing else to do yet
-                queries(tid, 128);
-                if (lane == 0) mbar_arrive(smem_u32(&q_first));
-            }
             const int rr = w.rr0 + row;
-            const bool active = rr < R, some = w.rr0 + warp * 32 < R;  // this row; any of the warp's
+            // this row; any of the warp's
+            const bool active = rr < R && row < chunk, some = w.rr0 + warp * 32 < R;
             const int full = min(max(base, 0), kend);  // keys every row sees
             const int32_t* bt = a.table + static_cast<size_t>(w.b) * a.max_blocks;
             unsigned long long vis = 0;  // of the new tokens, those this row sees
@@ -576,16 +553,17 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// [rows, heads, hd] of 16-bit elements, boxes of 64 dims of one head and `box` rows.
+// [rows, heads, hd] of 16-bit elements, boxes of 64 dims of `box_heads` heads and `box` rows.
 cudaError_t row_map(CUtensorMap* m, const void* base, int dtype, int hd, int heads, long long rows,
-                    int box) {
+                    int box_heads, int box) {
     const PFN_cuTensorMapEncodeTiled_v12000 enc = encode_fn();
     if (!enc) return cudaErrorNotSupported;
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(heads),
                                 static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(hd) * 2,
                                    static_cast<cuuint64_t>(heads) * hd * 2};
-    const cuuint32_t boxes[3] = {64, 1, static_cast<cuuint32_t>(box)}, ones[3] = {1, 1, 1};
+    const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box)};
+    const cuuint32_t ones[3] = {1, 1, 1};
     const CUresult r = enc(m, dtype == kBF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                            3, const_cast<void*>(base), dims, strides, boxes, ones,
                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -633,11 +611,13 @@ cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStre
         v = vo;
         src = {rt::KT, rps, p.a.batch * rps};
     }
-    CUtensorMap tk, tv;
-    cudaError_t e = row_map(&tk, k, c.dtype, c.hd, c.Hkv, src.rows, src.box);
-    if (e == cudaSuccess) e = row_map(&tv, v, c.dtype, c.hd, c.Hkv, src.rows, src.box);
+    const int G = p.a.Hq / c.Hkv;
+    CUtensorMap tq, tk, tv;
+    cudaError_t e = row_map(&tq, p.a.q, c.dtype, c.hd, p.a.Hq, p.a.total, G, rt::ROWS / G);
+    if (e == cudaSuccess) e = row_map(&tk, k, c.dtype, c.hd, c.Hkv, src.rows, 1, src.box);
+    if (e == cudaSuccess) e = row_map(&tv, v, c.dtype, c.hd, c.Hkv, src.rows, 1, src.box);
     if (e != cudaSuccess) return e;
-    void* args[] = {&tk, &tv, &p, &src};
+    void* args[] = {&tq, &tk, &tv, &p, &src};
     const void* f = bf ? (big ? reinterpret_cast<const void*>(&attn_rows_tc_kernel<__nv_bfloat16, 128>)
                               : reinterpret_cast<const void*>(&attn_rows_tc_kernel<__nv_bfloat16, 64>))
                        : (big ? reinterpret_cast<const void*>(&attn_rows_tc_kernel<__half, 128>)

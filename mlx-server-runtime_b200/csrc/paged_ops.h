@@ -55,7 +55,7 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& a, void* workspac
 // The tcgen05 form of the attention (paged_attn_tc.cu): 128 query rows and kRowsTcKeys keys
 // to a tile, over 16-bit rows; a quantised cache's are expanded into `expanded` first, which
 // takes rows_tc_expand_bytes for each sequence.
-constexpr int kRowsTcKeys = 64, kRowsTcThreads = 256;
+constexpr int kRowsTcKeys = 64, kRowsTcThreads = 224;
 namespace ra {
 struct Params;
 }

@@ -94,17 +94,18 @@ __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, i
 
 // A CTA's run of units as segments, each a range of tiles of one item. The first `extra`
 // CTAs take share + 1 units, the others share.
-template <int KT, int ROWS>
+template <int KT>
 struct Walk {
     int u, u_lo, u_hi, start;
-    int b, G, Hkv, share, extra, C, ch;
+    int b, G, Hkv, rows, share, extra, C, ch;
     // the segment
     Seq s;
     int g, rr0, t0, t1;
 
-    __device__ __forceinline__ void begin(const RowsArgs& a, int Hkv_, const Units& un, int parts,
-                                          int group, const int* pref) {
+    __device__ __forceinline__ void begin(const RowsArgs& a, int Hkv_, int rows_, const Units& un,
+                                          int parts, int group, const int* pref) {
         Hkv = Hkv_;
+        rows = rows_;
         G = a.Hq / Hkv;
         C = group;
         const int P = max(1, min(parts / C, un.total)), i = blockIdx.x / C;  // no share is empty
@@ -127,7 +128,7 @@ struct Walk {
     // Steps to the segment at u; false at the end of the run.
     __device__ __forceinline__ bool next(const RowsArgs& a) {
         while (u < u_hi) {
-            s = seq_of<KT>(a, b, G, ROWS);
+            s = seq_of<KT>(a, b, G, rows);
             const int n = (C > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
             if (u >= start + n) {
                 start += n;
@@ -151,7 +152,7 @@ struct Walk {
                 g = lone ? in : in >> 1;
                 chunk = !lone && (in & 1) ? s.chunks - 1 - pair : pair;
             }
-            rr0 = chunk * ROWS;
+            rr0 = chunk * rows;
             return true;
         }
         return false;
@@ -163,7 +164,7 @@ struct Walk {
     // ones every row sees, and the position of new token 0
     __device__ __forceinline__ int base() const { return s.L - s.n; }
     __device__ __forceinline__ int kend(const RowsArgs& a) const {
-        const int last = min(s.n * G, rr0 + ROWS) - 1;
+        const int last = min(s.n * G, rr0 + rows) - 1;
         return max(0, a.mask ? s.L : min(s.L, base() + last / G + 1));
     }
     // tiles of the segment that hold such keys
@@ -177,7 +178,7 @@ struct Walk {
     }
     __device__ __forceinline__ Cut cut() const {
         Cut c;
-        c.rows = min(s.n * G - rr0, ROWS);
+        c.rows = min(s.n * G - rr0, rows);
         c.slot = slot();
         c.last = owner(u - t0 + s.tiles - 1) * C + ch;
         c.step = C;
