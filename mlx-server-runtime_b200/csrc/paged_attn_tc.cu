@@ -68,6 +68,16 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
     return r;
 }
 
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};\n" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 // 3-D TMA load of one box (64 dims, one head, some rows); no cluster multicast.
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
                                             int x, int y, int z) {
@@ -78,6 +88,65 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 }  // namespace rt
+
+// One warp's 32 rows of O on their way out, whole (scaled, rounded to T, to their rows of the
+// output) or as a part (32-bit). They go by way of 2 KB of shared memory, 64 bytes of each at
+// a time, so that a store covers whole sectors: 16 bytes from each of 32 rows took 5000 to
+// 10000 cycles an item. Sixteen-byte chunks are swizzled: no bank conflicts. (Not inlined:
+// its registers would be the softmax's spills.)
+struct Leave {
+    uint32_t t_o;    // O's first column, or kNoCols: zeros
+    uint32_t stage;
+    int rows, x0, G, Hq;  // rows that are there, the first one's place in the chunk
+};
+constexpr uint32_t kNoCols = ~0u;
+
+template <typename T, int HD, bool WHOLE>
+__device__ __noinline__ void rows_leave(const Leave lv, float scale, void* base) {
+    using namespace rt;
+    constexpr int COLS = WHOLE ? 32 : 16;  // of O in 64 bytes
+    const int lane = threadIdx.x & 31, ch = lane & 3;
+    uint32_t off[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // a lane stores 16 bytes of rows lane / 4 + 8 i
+        const int r = 8 * i + (lane >> 2), x = lv.x0 + r, dn = x * (65536 / lv.G + 1) >> 16;
+        off[i] = WHOLE ? (dn * lv.Hq + x - dn * lv.G) * HD + ch * 8 : r * HD + ch * 4;
+    }
+#pragma unroll 1
+    for (int q = 0; q < HD / COLS; ++q) {
+        uint32_t v[COLS], o[16];
+        if (lv.t_o == kNoCols) {
+#pragma unroll
+            for (int x = 0; x < COLS; ++x) v[x] = 0u;
+        } else if constexpr (WHOLE) {
+            tmem_ld32(lv.t_o + q * COLS, v);
+        } else {
+            tmem_ld16(lv.t_o + q * COLS, v);
+        }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            if constexpr (WHOLE)
+                o[x] = pk_round<T>(__uint_as_float(v[2 * x]) * scale, __uint_as_float(v[2 * x + 1]) * scale);
+            else
+                o[x] = v[x];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            st_shared16(lv.stage + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4), o[4 * i], o[4 * i + 1],
+                        o[4 * i + 2], o[4 * i + 3]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 8 * i + (lane >> 2);
+            if (r < lv.rows) {
+                const uint4 d = ld_shared16(lv.stage + r * 64 + ((ch ^ (r >> 1 & 3)) << 4));
+                if constexpr (WHOLE) *reinterpret_cast<uint4*>(static_cast<T*>(base) + off[i] + q * COLS) = d;
+                else *reinterpret_cast<uint4*>(static_cast<float*>(base) + off[i] + q * COLS) = d;
+            }
+        }
+        __syncwarp();
+    }
+}
 
 // Where the 16-bit rows are: the cache's pages (box = page size), or the expanded rows of
 // sequence b from row b * rows_per_seq on, whole tiles of them, zeros behind the last key.
@@ -436,37 +505,22 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             if (any && !wait(pv_done, it - 1)) break;
             tc_fence_after();
             if (!some) continue;
-            const float inv = m == -INFINITY ? 0.f : 1.0f / l;
-            const size_t slot = static_cast<size_t>(w.slot()) * ROWS + row;
-            T* dst = nullptr;
-            if (active)
-                dst = static_cast<T*>(a.out) +
-                      (static_cast<size_t>(s.row0 + tok) * a.Hq + w.g * G + rr - tok * G) * HD;
-#pragma unroll 1
-            for (int q = 0; q < HD / 32; ++q) {
-                uint32_t v[32];
-                if (any) tmem_ld32(t_o + q * 32, v);
-                else
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) v[x] = 0u;
-                if (!active) continue;
-#pragma unroll
-                for (int x = 0; x < 32; x += 8) {
-                    float d[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) d[i] = __uint_as_float(v[x + i]);
-                    if (whole) {
-                        *reinterpret_cast<uint4*>(dst + q * 32 + x) =
-                            make_uint4(pk_round<T>(d[0] * inv, d[1] * inv), pk_round<T>(d[2] * inv, d[3] * inv),
-                                       pk_round<T>(d[4] * inv, d[5] * inv), pk_round<T>(d[6] * inv, d[7] * inv));
-                    } else {
-                        float4* o = reinterpret_cast<float4*>(p.part_o + slot * HD + q * 32 + x);
-                        o[0] = make_float4(d[0], d[1], d[2], d[3]);
-                        o[1] = make_float4(d[4], d[5], d[6], d[7]);
-                    }
-                }
+            Leave lv;
+            lv.t_o = any ? t_o : kNoCols;
+            lv.stage = smem_u32(smem + ROWS * HD * 2 + 4 * HB + warp * 2048);
+            lv.rows = min(min(R - w.rr0, chunk) - warp * 32, 32);
+            lv.x0 = warp * 32;
+            lv.G = G;
+            lv.Hq = a.Hq;
+            if (whole) {
+                rows_leave<T, HD, true>(lv, m == -INFINITY ? 0.f : 1.0f / l,
+                                        static_cast<T*>(a.out) +
+                                            (static_cast<size_t>(s.row0 + w.rr0 / G) * a.Hq + w.g * G) * HD);
+            } else {
+                const size_t slot = static_cast<size_t>(w.slot()) * ROWS + warp * 32;
+                rows_leave<T, HD, false>(lv, 1.f, p.part_o + slot * HD);
+                if (lane < lv.rows) p.part_ml[slot + lane] = make_float2(m, l);
             }
-            if (!whole && active) p.part_ml[slot] = make_float2(m, l);
         }
         if (row == 0) p.cut[blockIdx.x] = mine;
     }
@@ -571,8 +625,8 @@ cudaError_t row_map(CUtensorMap* m, const void* base, int dtype, int hd, int hea
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-size_t tc_smem(int hd) {  // Q, two tiles each of K and V, and the slack to align them
-    return (rt::ROWS + 4 * static_cast<size_t>(rt::KT)) * hd * 2 + 1024;
+size_t tc_smem(int hd) {  // Q, two tiles each of K and V, the epilogue's 8 KB, slack to align
+    return (rt::ROWS + 4 * static_cast<size_t>(rt::KT)) * hd * 2 + 8192 + 1024;
 }
 
 int rows_per_seq(const RowsArgs& a) { return (a.max_kv + rt::KT - 1) / rt::KT * rt::KT; }
