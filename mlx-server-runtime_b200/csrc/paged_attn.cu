@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
 
     zero_tail(a, HD, THREADS);
     const Units un = scan_units<KT>(a, Hkv, G, ROWS, p.group, pref);
-    Walk<KT> w;
+    Walk<KT, false> w;
     w.begin(a, Hkv, ROWS, un, p.parts, p.group, pref);
     Cut mine = {};
 

@@ -214,8 +214,10 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int page_shift = 31 - __clz(c.page);
-    Walk<KT> w;
-    w.begin(a, Hkv, chunk, un, p.parts, p.group, pref);
+    __shared__ Walk<KT, true> walks[THREADS / 32];
+    const Walk<KT, true>& w = walks[warp];
+    Steps<KT> steps = {walks[warp], a};
+    steps.begin(Hkv, chunk, un, p.parts, p.group, pref);
 
     // Tile j of the CTA's run uses buffer j & 1 of K, V, S and P, and that buffer's barriers'
     // phase j >> 1; item i the queries' barriers' phase i. No role is ever two phases behind
@@ -234,8 +236,8 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     auto step = [&]() -> bool {  // to the next tile; false behind the last
         if (++tile < te) return true;
         while (te >= 0) {
-            if (te > 0) w.advance();
-            if (!w.next(a)) {
+            if (te > 0) steps.advance();
+            if (!steps.next()) {
                 te = -1;
                 break;
             }
@@ -338,43 +340,42 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         const uint64_t vd = sw128_mnmajor_desc(smem_u32(vs), KT * 128);
         uint32_t ns = 0, npv = 0, nq = 0;  // S and P V issued, items of queries met
         uint32_t begins = 0;               // tiles that begin an item, by their last five bits
-        bool ok = true, more = true;
-        auto issue_s = [&]() {             // of the next tile, if there is one
-            if (!(more = step())) return;
+        bool more = step();                // a tile whose S is to come
+        while (more || npv < ns) {
+            // S runs up to two tiles ahead of P V. An item's first waits for its queries, and
+            // they for the last S of the item before: P V goes first then.
             const bool begin = tile == w.t0;
-            const uint32_t bit = 1u << (ns & 31), buf = ns & 1;
-            begins = begin ? begins | bit : begins & ~bit;
-            if ((begin && !spin(&q_full, nq++)) || !spin(k_full + buf, ns >> 1)) {
-                ok = false;
-                return;
-            }
-            tc_fence_after();
-            const uint64_t kb = kd + buf * (HB / 16);
-            const uint32_t d = tmem + buf * KT;
+            const uint32_t sb = ns & 1, vb = npv & 1;
+            if (more && ns - npv < 2 &&
+                (!begin || npv == ns ||
+                 (mbar_try_wait(smem_u32(&q_full), nq & 1) && mbar_try_wait(smem_u32(k_full + sb), ns >> 1 & 1)))) {
+                if ((begin && !spin(&q_full, nq++)) || !spin(k_full + sb, ns >> 1)) break;
+                tc_fence_after();
+                const uint32_t bit = 1u << (ns & 31);
+                begins = begin ? begins | bit : begins & ~bit;
+                const uint64_t kb = kd + sb * (HB / 16);
+                const uint32_t d = tmem + sb * KT;
 #pragma unroll
-            for (int i = 0; i < HD / 16; ++i)  // 16 dims: 32 bytes of a half of them
-                umma_f16_ss_by(leader, d, qd + (i / 4) * (ROWS * 128 / 16) + (i % 4) * 2,
-                               kb + (i / 4) * (KT * 128 / 16) + (i % 4) * 2, IDESC_S, i > 0 ? 1u : 0u);
-            umma_commit_by(leader, smem_u32(s_full + buf));
-            if (tile + 1 == te) umma_commit_by(leader, smem_u32(&q_free));
-            ++ns;
-        };
-        issue_s();
-        if (ok && more) issue_s();
-        while (ok && npv < ns) {
-            const uint32_t buf = npv & 1;
-            if (!spin(v_full + buf, npv >> 1) || !spin(p_full + buf, npv >> 1)) break;
+                for (int i = 0; i < HD / 16; ++i)  // 16 dims: 32 bytes of a half of them
+                    umma_f16_ss_by(leader, d, qd + (i / 4) * (ROWS * 128 / 16) + (i % 4) * 2,
+                                   kb + (i / 4) * (KT * 128 / 16) + (i % 4) * 2, IDESC_S, i > 0 ? 1u : 0u);
+                umma_commit_by(leader, smem_u32(s_full + sb));
+                if (tile + 1 == te) umma_commit_by(leader, smem_u32(&q_free));
+                ++ns;
+                more = step();
+                continue;
+            }
+            if (!spin(v_full + vb, npv >> 1) || !spin(p_full + vb, npv >> 1)) break;
             tc_fence_after();
-            const uint64_t vb = vd + buf * (HB / 16);
-            const uint32_t pa = tmem + buf * KT;
-            const bool begin = begins >> (npv & 31) & 1;
+            const uint64_t vt = vd + vb * (HB / 16);
+            const uint32_t pa = tmem + vb * KT;
+            const bool fresh = begins >> (npv & 31) & 1;
 #pragma unroll
             for (int i = 0; i < KT / 16; ++i)  // 16 keys: 8 columns of P, 2 KB of V
-                umma_f16_ts_by(leader, tmem + kOCol, pa + 8 * i, vb + i * (2048 / 16), IDESC_O,
-                               (!begin || i > 0) ? 1u : 0u);
-            umma_commit_by(leader, smem_u32(pv_done + buf));
+                umma_f16_ts_by(leader, tmem + kOCol, pa + 8 * i, vt + i * (2048 / 16), IDESC_O,
+                               (!fresh || i > 0) ? 1u : 0u);
+            umma_commit_by(leader, smem_u32(pv_done + vb));
             ++npv;
-            if (more) issue_s();
         }
         // every product issued has finished before tensor memory is freed
         umma_commit_by(leader, smem_u32(&drained));
@@ -387,8 +388,8 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         uint32_t it = 0;  // tiles so far
         Cut mine = {};
         bool ok = true;
-        for (; ok && w.next(a); w.advance()) {
-            const Seq& s = w.s;
+        for (; ok && steps.next(); steps.advance()) {
+            const Seq s = w.s;
             const int kend = w.kend(a), te = w.tile_end(a), base = w.base(), R = s.n * G;
             const int rr = w.rr0 + row;
             // this row; any of the warp's

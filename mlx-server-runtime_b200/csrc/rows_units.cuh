@@ -94,10 +94,17 @@ __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, i
 
 // A CTA's run of units as segments, each a range of tiles of one item. The first `extra`
 // CTAs take share + 1 units, the others share.
-template <int KT>
+// STEPS: items of a sequence follow one another without a division or a load, from more
+// words of state: for the specialised warps of the tcgen05 kernel, each with a walk of its
+// own in shared memory that its lane 0 moves (see Steps). Otherwise every item is worked out
+// anew, from state that the compiler keeps off the main loop's registers (those words would
+// be its spills: 32 sequences' decode step 91 -> 105 us).
+template <int KT, bool STEPS>
 struct Walk {
     int u, u_lo, u_hi, start;
     int b, G, Hkv, rows, share, extra, C, ch;
+    bool known;  // s is sequence b, whose units end at `end`
+    int end, pair, in;
     // the segment
     Seq s;
     int g, rr0, t0, t1;
@@ -113,6 +120,7 @@ struct Walk {
         share = un.total / P;
         extra = un.total - share * P;
         u = u_lo = u_hi = start = b = 0;
+        if (STEPS) known = false;
         if (i >= P || un.total == 0) return;
         u = u_lo = i * share + min(i, extra);
         u_hi = u + share + (i < extra ? 1 : 0);
@@ -128,26 +136,45 @@ struct Walk {
     // Steps to the segment at u; false at the end of the run.
     __device__ __forceinline__ bool next(const RowsArgs& a) {
         while (u < u_hi) {
-            s = seq_of<KT>(a, b, G, rows);
-            const int n = (C > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
-            if (u >= start + n) {
-                start += n;
+            if (!STEPS || !known) {
+                s = seq_of<KT>(a, b, G, rows);
+                const int n = (C > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
+                if (u >= start + n) {
+                    start += n;
+                    ++b;
+                    continue;
+                }
+                if (C > 1 && ch >= s.chunks) {  // no rows of this sequence for this CTA
+                    u = min(u_hi, start + n);
+                    continue;
+                }
+                if (STEPS) {
+                    known = true;
+                    end = start + n;
+                }
+                const int item = (u - start) / s.tiles;
+                t0 = (u - start) - item * s.tiles;
+                pair = C > 1 ? 0 : item / (2 * Hkv);
+                in = item - pair * 2 * Hkv;
+            } else if (u >= end) {
+                start = end;
                 ++b;
+                known = false;
                 continue;
+            } else {
+                t0 = 0;  // (a segment that ends before its item is the run's last)
+                ++in;
+                if (C == 1 && in == 2 * Hkv) {
+                    in = 0;
+                    ++pair;
+                }
             }
-            if (C > 1 && ch >= s.chunks) {  // no rows of this sequence for this CTA
-                u = min(u_hi, start + n);
-                continue;
-            }
-            const int item = (u - start) / s.tiles;
-            t0 = (u - start) - item * s.tiles;
             t1 = min(s.tiles, t0 + (u_hi - u));
             int chunk = ch;
-            g = item;
+            g = in;
             if (C == 1) {
                 // The chunks in pairs from both ends: a causal mask leaves the first ones
                 // fewer keys than the last, and a run of items then has its share of both
-                const int pair = item / (2 * Hkv), in = item - pair * 2 * Hkv;
                 const bool lone = 2 * pair + 1 == s.chunks;
                 g = lone ? in : in >> 1;
                 chunk = !lone && (in & 1) ? s.chunks - 1 - pair : pair;
@@ -186,6 +213,30 @@ struct Walk {
         c.rr0 = rr0;
         c.g = g;
         return c;
+    }
+};
+
+// A warp's way of moving its Walk: every lane calls, lane 0 moves.
+template <int KT>
+struct Steps {
+    Walk<KT, true>& w;
+    const RowsArgs& a;
+    __device__ __forceinline__ void begin(int Hkv, int rows, const Units& un, int parts, int group,
+                                          const int* pref) {
+        if ((threadIdx.x & 31) == 0) w.begin(a, Hkv, rows, un, parts, group, pref);
+        __syncwarp();
+    }
+    __device__ __forceinline__ bool next() {
+        int r = 0;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) r = w.next(a);
+        __syncwarp();
+        return __shfl_sync(0xffffffffu, r, 0) != 0;
+    }
+    __device__ __forceinline__ void advance() {
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) w.advance();
+        __syncwarp();
     }
 };
 
