@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
     T* out = static_cast<T*>(a.out);
 
     zero_tail(a, HD, THREADS);
-    const Units un = scan_units<KT>(a, Hkv, G, ROWS, p.group, pref);
-    Walk<KT, false> w;
+    const Units un = scan_units<KT, true>(a, Hkv, G, ROWS, p.group, pref);
+    Walk<KT, false, true> w;
     w.begin(a, Hkv, ROWS, un, p.parts, p.group, pref);
     Cut mine = {};
 
@@ -527,18 +527,16 @@ Plan plan_of(const KvCache& c, const RowsArgs& a) {
     p.rows = p.tc ? 128 : r > 8 ? 16 : 8;
     p.chunk = p.tc ? 128 / G * G : p.rows;
     p.kt = p.tc ? kRowsTcKeys : ra::KT;
-    // CTAs the units are shared out to: what the GPU holds at once, at most one per unit
+    // CTAs the units are shared out to, in groups that take the same ones: what the GPU holds
+    // at once, at most a group per unit
     const long long most = 148LL * (p.tc ? 2 : ra::resident(c.hd, c.bits, p.rows / 8));
-    const long long tiles = (a.max_kv + p.kt - 1) / p.kt;
-    long long units = (r + p.chunk - 1) / p.chunk * (tiles > 0 ? tiles : 1) * c.Hkv;
-    units = units < most ? units * a.batch : most;
-    p.parts = static_cast<int>(units < 1 ? 1 : units < most ? units : most);
-    // up to eight chunks go side by side
-    const int chunks = static_cast<int>((r + p.chunk - 1) / p.chunk);
-    p.group = p.tc && chunks >= 2 && chunks <= 8 ? chunks : 1;
-    if (p.group > 1) p.parts = (p.parts + p.group - 1) / p.group * p.group > most
-                                   ? static_cast<int>(most / p.group * p.group)
-                                   : (p.parts + p.group - 1) / p.group * p.group;
+    const long long tiles = a.max_kv > 0 ? (a.max_kv + p.kt - 1) / p.kt : 1;
+    const long long chunks = (r + p.chunk - 1) / p.chunk;
+    p.group = !p.tc ? c.Hkv : chunks >= 2 && chunks <= 8 ? static_cast<int>(chunks) : 1;
+    long long units = tiles * (p.tc ? c.Hkv * (p.group > 1 ? 1 : chunks) : 1);  // of a sequence
+    long long groups = most / p.group > 1 ? most / p.group : 1;
+    if (units < groups && units * a.batch < groups) groups = units * a.batch > 1 ? units * a.batch : 1;
+    p.parts = static_cast<int>(groups * p.group);
     return p;
 }
 
@@ -649,7 +647,7 @@ cudaError_t launch_attn_rows(const KvCache& c, const RowsArgs& all, void* worksp
         }
         if (e != cudaSuccess) return e;
         overlap = true;  // (from here on every launch waits for the one before)
-        if (pl.parts == 1) continue;
+        if (pl.parts == pl.group) continue;  // (one run of units: nothing is cut)
         const void* fc = bf ? (big ? combine_fn<__nv_bfloat16, 128>(pl.rows)
                                    : combine_fn<__nv_bfloat16, 64>(pl.rows))
                             : (big ? combine_fn<__half, 128>(pl.rows) : combine_fn<__half, 64>(pl.rows));

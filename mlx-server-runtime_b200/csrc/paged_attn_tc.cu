@@ -208,14 +208,14 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
     const KvCache& c = p.c;
     const int Hkv = c.Hkv, G = a.Hq / Hkv, chunk = ROWS / G * G;
     zero_tail(a, HD, THREADS);
-    const Units un = scan_units<KT>(a, Hkv, G, chunk, p.group, pref);
+    const Units un = scan_units<KT, false>(a, Hkv, G, chunk, p.group, pref);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const int page_shift = 31 - __clz(c.page);
-    __shared__ Walk<KT, true> walks[THREADS / 32];
-    const Walk<KT, true>& w = walks[warp];
+    __shared__ Walk<KT, true, false> walks[THREADS / 32];
+    const Walk<KT, true, false>& w = walks[warp];
     Steps<KT> steps = {walks[warp], a};
     steps.begin(Hkv, chunk, un, p.parts, p.group, pref);
 

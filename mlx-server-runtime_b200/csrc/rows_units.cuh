@@ -3,9 +3,10 @@
 // items as one sequence of units that the CTAs take in equal contiguous runs. Or, with few
 // chunks (a tree's), the tiles of all (sequence, kv head) items, of which C CTAs take the
 // same run, each another chunk: they read the same keys at about the same time, so that all
-// but one find them in L2 (16 trees of 64 tokens over 8192 16-bit keys, 448 rows in four
-// chunks over 168 MB: 127 us with the chunks as units of their own). And how the parts of an item that
-// several CTAs computed are joined.
+// but one find them in L2. Or, with one chunk (a decode step), the tiles of all sequences, of
+// which Hkv CTAs take the same run, each another head: a sector of scales holds several
+// heads' (taken head after head, 32 sequences of up to 16384 4-bit keys read 295 MB for the
+// 193 they hold). And how the parts of an item that several CTAs computed are joined.
 #pragma once
 
 #include "common.cuh"
@@ -31,7 +32,7 @@ struct Params {
     float2* part_ml;  // [2 P][ROWS] maximum (base 2) and sum
     Cut* cut;         // [P]
     int parts;        // P: CTAs, of which each run of `group` takes the same units
-    int group;        // C: 1, or the most chunks of a sequence, each CTA of the run one of them
+    int group;        // C: 1, the most chunks of a sequence, or its heads: each CTA takes one
 };
 
 // One sequence's place in the batch, with everything a bad length or offset could do bounded.
@@ -61,7 +62,7 @@ struct Units {
     int total;
     int per;  // sequences per scanning thread
 };
-template <int KT>
+template <int KT, bool HEADS>
 __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, int rows, int group,
                                             int* pref /* shared [SCAN + 1] */) {
     __shared__ int wsum[SCAN / 32];
@@ -72,7 +73,8 @@ __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, i
     if (tid < SCAN) {
         for (int b = tid * u.per; b < min(a.batch, (tid + 1) * u.per); ++b) {
             const Seq s = seq_of<KT>(a, b, G, rows);
-            inc += (group > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
+            inc += HEADS ? min(s.chunks, 1) * s.tiles
+                         : (group > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -99,7 +101,8 @@ __device__ __forceinline__ Units scan_units(const RowsArgs& a, int Hkv, int G, i
 // own in shared memory that its lane 0 moves (see Steps). Otherwise every item is worked out
 // anew, from state that the compiler keeps off the main loop's registers (those words would
 // be its spills: 32 sequences' decode step 91 -> 105 us).
-template <int KT, bool STEPS>
+// HEADS: one chunk to a sequence, and the CTAs of a run take its heads.
+template <int KT, bool STEPS, bool HEADS>
 struct Walk {
     int u, u_lo, u_hi, start;
     int b, G, Hkv, rows, share, extra, C, ch;
@@ -138,13 +141,14 @@ struct Walk {
         while (u < u_hi) {
             if (!STEPS || !known) {
                 s = seq_of<KT>(a, b, G, rows);
-                const int n = (C > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
+                const int n = HEADS ? min(s.chunks, 1) * s.tiles
+                                    : (C > 1 ? min(s.chunks, 1) : s.chunks) * s.tiles * Hkv;
                 if (u >= start + n) {
                     start += n;
                     ++b;
                     continue;
                 }
-                if (C > 1 && ch >= s.chunks) {  // no rows of this sequence for this CTA
+                if (!HEADS && C > 1 && ch >= s.chunks) {  // no rows of this sequence for this CTA
                     u = min(u_hi, start + n);
                     continue;
                 }
@@ -152,7 +156,7 @@ struct Walk {
                     known = true;
                     end = start + n;
                 }
-                const int item = (u - start) / s.tiles;
+                const int item = HEADS ? 0 : (u - start) / s.tiles;
                 t0 = (u - start) - item * s.tiles;
                 pair = C > 1 ? 0 : item / (2 * Hkv);
                 in = item - pair * 2 * Hkv;
@@ -170,6 +174,11 @@ struct Walk {
                 }
             }
             t1 = min(s.tiles, t0 + (u_hi - u));
+            if (HEADS) {
+                g = ch;
+                rr0 = 0;
+                return true;
+            }
             int chunk = ch;
             g = in;
             if (C == 1) {
@@ -219,7 +228,7 @@ struct Walk {
 // A warp's way of moving its Walk: every lane calls, lane 0 moves.
 template <int KT>
 struct Steps {
-    Walk<KT, true>& w;
+    Walk<KT, true, false>& w;
     const RowsArgs& a;
     __device__ __forceinline__ void begin(int Hkv, int rows, const Units& un, int parts, int group,
                                           const int* pref) {
