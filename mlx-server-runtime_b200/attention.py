@@ -74,6 +74,9 @@ class QuantizedKV:
             raise ValueError("a quantized cache's tensors must be contiguous")
         if c.device != s.device or c.device != b.device:
             raise ValueError("a quantized cache's tensors must be on one device")
+        # the C ABI's fields: every call compares and passes them
+        object.__setattr__(self, "_geometry", (*c.shape[:3], s.shape[3] * self.group_size,
+                                               self.bits, self.group_size, _DT[s.dtype]))
 
     @classmethod
     def zeros(cls, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
@@ -103,14 +106,11 @@ class QuantizedKV:
 def _kv_struct(k, v) -> _lib.KVCache:
     """The C ABI's view of one layer's pools (16-bit tensors, or QuantizedKV)."""
     if isinstance(k, QuantizedKV):
-        if not isinstance(v, QuantizedKV) or v.codes.shape != k.codes.shape or \
-                v.scales.shape != k.scales.shape or v.bits != k.bits or v.dtype != k.dtype:
+        if not isinstance(v, QuantizedKV) or v._geometry != k._geometry:
             raise ValueError("keys and values must share a quantized cache's shape and width")
-        pages, page, hkv = k.codes.shape[:3]
         return _lib.KVCache(k.codes.data_ptr(), v.codes.data_ptr(), k.scales.data_ptr(),
-                            k.biases.data_ptr(), v.scales.data_ptr(), v.biases.data_ptr(), pages,
-                            page, hkv, k.scales.shape[3] * k.group_size, k.bits, k.group_size,
-                            _DT[k.dtype])
+                            k.biases.data_ptr(), v.scales.data_ptr(), v.biases.data_ptr(),
+                            *k._geometry)
     shape, dt = k.shape, k.dtype
     if isinstance(v, QuantizedKV) or v.shape != shape or v.dtype is not dt:
         raise ValueError("k_cache and v_cache must share shape and dtype")
@@ -267,26 +267,27 @@ def _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, 
                     tree_mask, scale, what):
     """mlxq_paged_attention_rows: a cache of any width, one or several rows a sequence."""
     kv = _kv_struct(k_cache, v_cache)
-    if q.ndim != 3 or q.dtype != k_cache.dtype or q.shape[2] != kv.head_dim:
+    shape = q.shape
+    if len(shape) != 3 or _DT.get(q.dtype) != kv.dtype or shape[2] != kv.head_dim:
         raise ValueError("q must be [rows, n_heads, head_dim] of the cache's head_dim and dtype")
+    rows, H, _ = shape
     q = q.contiguous()
     block_table, kv_lens = _i32(block_table, "block_table"), _i32(kv_lens, "kv_lens")
-    if block_table.ndim != 2 or kv_lens.shape != (block_table.shape[0],):
+    if block_table.dim() != 2 or kv_lens.dim() != 1 or kv_lens.numel() != block_table.size(0):
         raise ValueError("block_table must be [B, max_blocks] and kv_lens [B]")
-    B = block_table.shape[0]
+    B, blocks = block_table.shape
     if cu_q is not None:
         cu_q = _i32(cu_q, "cu_q")
-        if cu_q.shape != (B + 1,):
+        if cu_q.dim() != 1 or cu_q.numel() != B + 1:
             raise ValueError(f"cu_q must be [{B + 1}] (one offset per sequence, then the total)")
-    elif q.shape[0] != B:
-        raise ValueError(f"q must have one row per sequence ({B}), got {q.shape[0]}")
+    elif rows != B:
+        raise ValueError(f"q must have one row per sequence ({B}), got {rows}")
     if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.shape != (q.shape[0],):
-            raise ValueError(f"tree_mask must be int64 [{q.shape[0]}]")
+        if tree_mask.dtype is not torch.int64 or tree_mask.dim() != 1 or tree_mask.numel() != rows:
+            raise ValueError(f"tree_mask must be int64 [{rows}]")
         tree_mask = tree_mask.contiguous()
     dev = _on(q, cu_q, _pool(k_cache), _pool(v_cache), block_table, kv_lens, tree_mask)
     out = torch.empty_like(q)
-    rows, H, _ = q.shape
     max_q_len, max_kv_len = int(max_q_len), int(max_kv_len)
     L = _lib.load()
 
@@ -297,7 +298,7 @@ def _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, 
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
         return L.mlxq_paged_attention_rows(
             kv, q.data_ptr(), None if cu_q is None else cu_q.data_ptr(), rows, max_q_len,
-            block_table.data_ptr(), block_table.shape[1], kv_lens.data_ptr(), max_kv_len,
+            block_table.data_ptr(), blocks, kv_lens.data_ptr(), max_kv_len,
             None if tree_mask is None else tree_mask.data_ptr(), out.data_ptr(), B, H,
             float(scale), None if ws is None else ws.data_ptr(), need, st)
 
