@@ -42,7 +42,9 @@ __device__ __forceinline__ uint2 ld8(const void* p) { return *reinterpret_cast<c
 //   (y_i, y_{i+hd/2}) -> (y_i cos - y_{i+hd/2} sin, y_i sin + y_{i+hd/2} cos), rounded to T
 // The angle is position * turns[i] reduced to one turn in 64 bits (at position 10^5 a
 // 32-bit product is off by several 2^-8 rad, more than the rounding of the result), then
-// 32-bit sine and cosine of the rest. In a quantised cache the row rounded to T is
+// 32-bit sine and cosine of the rest, one pair to a thread and through shared memory to the
+// CTA's warps: worked out by every warp for itself, they were a third of the instructions,
+// which is what bounds a prompt's append. In a quantised cache the row rounded to T is
 // quantised by quantize()'s rule: a group's least and largest value by shuffles over its
 // lanes, four codes per lane and half.
 template <typename T, int HD, int BITS>
@@ -52,18 +54,17 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int li = lane % LPH, e0 = 4 * li;
     const KvCache& c = a.c;
-    double turn[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) turn[j] = a.turns[e0 + j];
+    __shared__ float4 cos4[HALF / 4], sin4[HALF / 4];
     const T* qn = static_cast<const T*>(a.q_norm);
     const T* kn = static_cast<const T*>(a.k_norm);
     pdl_wait();
     const int t = blockIdx.x;
     const int slot = a.slots[t];
-    const double pos = static_cast<double>(a.positions[t]);
     const bool keep = slot >= 0 && slot < c.pages * static_cast<long long>(c.page);
     const int heads = a.Hq + 2 * c.Hkv;
-    const int first = (blockIdx.y * (blockDim.x >> 5) + warp) * a.rounds * HPW + lane / LPH;
+    // groups of heads in turn, so that the warps share the heads that are quantised
+    const int stride = gridDim.y * (blockDim.x >> 5) * HPW;
+    const int first = (blockIdx.y * (blockDim.x >> 5) + warp) * HPW + lane / LPH;
     const T* src = static_cast<const T*>(a.qkv) + t * a.ld;
     uint2 next[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)};
     auto fetch = [&](int h) {  // a head's elements, a round before they are used
@@ -73,17 +74,22 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
         }
     };
     fetch(first);
-    float cs[4], sn[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const double x = pos * turn[j];
-        sincospif(2.0f * static_cast<float>(x - rint(x)), &sn[j], &cs[j]);
+    const double pos = static_cast<double>(a.positions[t]);
+    for (int i = threadIdx.x; i < HALF; i += blockDim.x) {
+        const double x = pos * a.turns[i];
+        float sine, cosine;
+        sincospif(2.0f * static_cast<float>(x - rint(x)), &sine, &cosine);
+        reinterpret_cast<float*>(cos4)[i] = cosine;
+        reinterpret_cast<float*>(sin4)[i] = sine;
     }
+    __syncthreads();
+    const float cs[4] = {cos4[li].x, cos4[li].y, cos4[li].z, cos4[li].w};
+    const float sn[4] = {sin4[li].x, sin4[li].y, sin4[li].z, sin4[li].w};
     for (int r = 0; r < a.rounds; ++r) {
-        const int h = first + r * HPW;
+        const int h = first + r * stride;
         const bool live = h < heads;
         uint2 lo = next[0], hi = next[1];
-        if (r + 1 < a.rounds) fetch(h + HPW);
+        if (r + 1 < a.rounds) fetch(h + stride);
         float x[4] = {Elem<T>::lo(lo.x), Elem<T>::hi(lo.x), Elem<T>::lo(lo.y), Elem<T>::hi(lo.y)};
         float y[4] = {Elem<T>::lo(hi.x), Elem<T>::hi(hi.x), Elem<T>::lo(hi.y), Elem<T>::hi(hi.y)};
         const bool is_q = h < a.Hq, is_v = h >= a.Hq + c.Hkv;
@@ -145,23 +151,30 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
                 mx[0] = mx[1] = fmaxf(mx[0], mx[1]);
             }
             const int seg = min(LPH, c.gs / 4);  // lanes of a group
-            for (int o = seg >> 1; o > 0; o >>= 1)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    mn[s] = fminf(mn[s], __shfl_xor_sync(0xffffffffu, mn[s], o));
-                    mx[s] = fmaxf(mx[s], __shfl_xor_sync(0xffffffffu, mx[s], o));
-                }
+            // even lanes go on with the lower half's group, odd lanes with the upper half's
+            const int side = li & 1;
+            float lo_s = fminf(mn[side], __shfl_xor_sync(0xffffffffu, mn[side ^ 1], 1));
+            float hi_s = fmaxf(mx[side], __shfl_xor_sync(0xffffffffu, mx[side ^ 1], 1));
+            for (int o = seg >> 1; o > 1; o >>= 1) {
+                lo_s = fminf(lo_s, __shfl_xor_sync(0xffffffffu, lo_s, o));
+                hi_s = fmaxf(hi_s, __shfl_xor_sync(0xffffffffu, hi_s, o));
+            }
             constexpr float n_bins = static_cast<float>((1 << BITS) - 1);
-            float sc[2], bi[2];
+            float sc[2], bi[2], rc[2];
+            quant_group(lo_s, hi_s, n_bins, sc[0], bi[0]);
+            rc[0] = __frcp_rn(sc[0]);
+            sc[1] = __shfl_xor_sync(0xffffffffu, sc[0], 1);
+            bi[1] = __shfl_xor_sync(0xffffffffu, bi[0], 1);
+            rc[1] = __shfl_xor_sync(0xffffffffu, rc[0], 1);
             uint32_t code[2] = {0u, 0u};
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                quant_group(mn[s], mx[s], n_bins, sc[s], bi[s]);
-                const float r = __frcp_rn(sc[s]);
+            for (int s = 0; s < 2; ++s) {  // this half's: the lane's own, or its neighbour's
+                const float scale = side == s ? sc[0] : sc[1], bias = side == s ? bi[0] : bi[1];
+                const float r = side == s ? rc[0] : rc[1];
                 const bool fast = fabsf(r) >= 0x1p-126f && fabsf(r) <= 0x1p126f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    code[s] |= quant_code(__fsub_rn(s ? q[j] : p[j], bi[s]), sc[s], r, n_bins, fast)
+                    code[s] |= quant_code(__fsub_rn(s ? q[j] : p[j], bias), scale, r, n_bins, fast)
                                << (BITS * j);
             }
             uint32_t* words = static_cast<uint32_t*>(is_v ? c.v : c.k) + row * (HD * BITS / 32);
@@ -178,16 +191,11 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
                 const uint32_t word = odd ? (got | code[1] << 16) : (code[0] | got << 16);
                 if (put) words[(odd ? HALF / 8 : 0) + li / 2] = word;
             }
-            if (put && (li & (seg - 1)) == 0) {
-                const int ng = HD / c.gs;
-                T* sd = static_cast<T*>(is_v ? c.vs : c.ks) + row * ng;
-                T* bd = static_cast<T*>(is_v ? c.vb : c.kb) + row * ng;
-                sd[e0 / c.gs] = Elem<T>::from_f(sc[0]);
-                bd[e0 / c.gs] = Elem<T>::from_f(bi[0]);
-                if (!whole) {
-                    sd[(HALF + e0) / c.gs] = Elem<T>::from_f(sc[1]);
-                    bd[(HALF + e0) / c.gs] = Elem<T>::from_f(bi[1]);
-                }
+            // the first two lanes of a group hold its halves' scales and biases
+            if (put && (li & (seg - 1)) < 2 && !(whole && side)) {
+                const size_t at = row * (HD / c.gs) + (side ? HALF + e0 - 4 : e0) / c.gs;
+                static_cast<T*>(is_v ? c.vs : c.ks)[at] = Elem<T>::from_f(sc[0]);
+                static_cast<T*>(is_v ? c.vb : c.kb)[at] = Elem<T>::from_f(bi[0]);
             }
         }
     }
@@ -241,8 +249,8 @@ cudaError_t launch_norm_rope_append(const KvCache& c, const void* qkv, long long
     const int want = 148 * 16;
     int rounds = 1;
     while (rounds < 8 && static_cast<long long>(tokens) * groups / (2 * rounds) >= want) rounds *= 2;
-    a.rounds = rounds;
     const int warps = (groups + rounds - 1) / rounds;
+    a.rounds = (groups + warps - 1) / warps;  // (evened out)
     const int wpc = warps < 4 ? warps : 4;
     void* args[] = {&a};
     static PerDevice cfg[12];
