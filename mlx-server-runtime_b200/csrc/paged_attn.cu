@@ -61,8 +61,10 @@ __device__ __forceinline__ void ldw(const void* at, uint32_t (&r)[N]) {
 }
 
 // CTAs of an SM: what the registers of a variant allow (and the launch bounds ask for).
+// Three rather than four for 4 bits and heads of 128, which spills nothing: 32 sequences of
+// up to 16384 keys 80 us (four: 78), one of 32768 19 (22), 64 of 1000 24 (29).
 constexpr int resident(int hd, int bits, int nt) {
-    return nt == 2 ? 2 : bits == 16 ? (hd == 64 ? 3 : 2) : hd == 64 || bits == 4 ? 4 : 3;
+    return nt == 2 ? 2 : bits == 16 ? (hd == 64 ? 3 : 2) : hd == 64 ? 4 : 3;
 }
 }  // namespace ra
 
@@ -535,6 +537,10 @@ Plan plan_of(const KvCache& c, const RowsArgs& a) {
     p.group = !p.tc ? c.Hkv : chunks >= 2 && chunks <= 8 ? static_cast<int>(chunks) : 1;
     long long units = tiles * (p.tc ? c.Hkv * (p.group > 1 ? 1 : chunks) : 1);  // of a sequence
     long long groups = most / p.group > 1 ? most / p.group : 1;
+    // runs of fewer than four tiles cost more to join than they save: two CTAs an SM then
+    // (a sequence of 32768 4-bit keys 17 us, with three 19; 16 of 4097 17 and 19)
+    const long long few = 296 / p.group;
+    if (!p.tc && units * a.batch < 4 * groups && few < groups) groups = few > 1 ? few : 1;
     if (units < groups && units * a.batch < groups) groups = units * a.batch > 1 ? units * a.batch : 1;
     p.parts = static_cast<int>(groups * p.group);
     return p;
