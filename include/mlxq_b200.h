@@ -413,7 +413,8 @@ typedef struct mlxq_kv_cache {
  * dtype; NULL leaves that side as it is): the head norms of Qwen3-style attention
  * (models/qwen3.py of the reference). Norm and rotation are one 32-bit
  * computation rounded once; the angle is reduced in 64 bits. With bits 8 or 4 the rounded
- * rows are quantized as mlxq_quantize would quantize them. Slots outside
+ * rows are quantized by mlxq_quantize's rule, but for a group's range, which is multiplied by
+ * the 32-bit reciprocal of its steps (15 or 255) rather than divided by them. Slots outside
  * [0, num_pages * page_size) are skipped; two tokens of one call must not share a slot.
  */
 int mlxq_norm_rope_kv_append(const mlxq_kv_cache* cache, const void* qkv, int64_t ld, void* q_out,

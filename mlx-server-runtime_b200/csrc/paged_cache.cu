@@ -45,7 +45,7 @@ __device__ __forceinline__ uint2 ld8(const void* p) { return *reinterpret_cast<c
 // 32-bit sine and cosine of the rest, one pair to a thread and through shared memory to the
 // CTA's warps: worked out by every warp for itself, they were a third of the instructions,
 // which is what bounds a prompt's append. In a quantised cache the row rounded to T is
-// quantised by quantize()'s rule: a group's least and largest value by shuffles over its
+// quantised by quantize()'s rule (see quant_group): a group's least and largest value by shuffles over its
 // lanes, four codes per lane and half.
 template <typename T, int HD, int BITS>
 __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_constant__ AppendArgs a) {
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
             }
             constexpr float n_bins = static_cast<float>((1 << BITS) - 1);
             float sc[2], bi[2], rc[2];
-            quant_group(lo_s, hi_s, n_bins, sc[0], bi[0]);
+            quant_group(lo_s, hi_s, __fmul_rn(__fsub_rn(hi_s, lo_s), 1.0f / n_bins), sc[0], bi[0]);
             rc[0] = __frcp_rn(sc[0]);
             sc[1] = __shfl_xor_sync(0xffffffffu, sc[0], 1);
             bi[1] = __shfl_xor_sync(0xffffffffu, bi[0], 1);

@@ -1,5 +1,5 @@
-// The group-wise affine quantization rule, shared by quantize_kernel and the kernels that
-// write a quantized KV cache, so that both give the same codes, scales and biases.
+// The group-wise affine quantization rule, shared by quantize_kernel and the kernel that
+// writes a quantized KV cache.
 #pragma once
 
 #include "common.cuh"
@@ -28,13 +28,16 @@ __device__ __forceinline__ uint32_t quant_code(float d, float s, float r, float 
     return __float_as_uint(__fadd_rn(k, kRoundMagic)) - kRoundMagicBits;
 }
 
-// Scale and bias of a group from its least and largest value: the end of larger
-// magnitude is kept exactly (bias = that end, scale = end / code of zero).
-__device__ __forceinline__ void quant_group(float lmin, float lmax, float n_bins, float& scale,
+// Scale and bias of a group from its least and largest value and a first step, its range
+// over the number of steps: the end of larger magnitude is kept exactly (bias = that end,
+// scale = end / code of zero). quantize_kernel divides for the step; the cache multiplies by
+// the steps' reciprocal, a division fewer. The two can differ in the step's last bit, which
+// decides where the end lies half way between two codes from zero (ends of one magnitude, for
+// one): either neighbour then serves.
+__device__ __forceinline__ void quant_group(float lmin, float lmax, float step, float& scale,
                                             float& bias) {
     const bool mask = fabsf(lmin) > fabsf(lmax);
-    scale = __fdiv_rn(__fsub_rn(lmax, lmin), n_bins);
-    scale = fmaxf(scale, 1e-7f);
+    scale = fmaxf(step, 1e-7f);
     scale = mask ? scale : -scale;
     const float edge = mask ? lmin : lmax;
     const float q0 = rintf(__fdiv_rn(edge, scale));

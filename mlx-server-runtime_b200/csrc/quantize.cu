@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ w,
     if (!live) return;
 
     float scale, bias;
-    quant_group(lmin, lmax, n_bins, scale, bias);
+    quant_group(lmin, lmax, __fdiv_rn(__fsub_rn(lmax, lmin), n_bins), scale, bias);
     const float r = __frcp_rn(scale);
     const float ar = fabsf(r);
     const bool fast = ar >= 0x1p-126f && ar <= 0x1p126f;

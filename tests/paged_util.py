@@ -34,6 +34,28 @@ def rotate_bound(ref, mag, t):
     return U[t] * ref.abs() + (68 + 32) * F * mag + (2.0 ** -24 if t == torch.float16 else 0.0)
 
 
+def quantized(x, gs, bits):
+    """Codes (packed from the low bits up), scales and biases of rows x [..., hd] of a 16-bit
+    type by the cache's rule, in 32-bit arithmetic on the CPU: a step = range * (1 / steps),
+    the end of larger magnitude kept exactly."""
+    t = x.dtype
+    v = x.cpu().float().unflatten(-1, (-1, gs))
+    hi, lo = v.amax(-1), v.amin(-1)
+    steps = torch.tensor(float(2 ** bits - 1))
+    neg = lo.abs() > hi.abs()
+    s = ((hi - lo) * (1.0 / steps)).clamp_min(1e-7)
+    s = torch.where(neg, s, -s)
+    edge = torch.where(neg, lo, hi)
+    q0 = torch.round(edge / s)
+    s = torch.where(q0 != 0, edge / torch.where(q0 != 0, q0, 1.0), s)
+    b = torch.where(q0 != 0, edge, 0.0)
+    q = torch.round((v - b[..., None]) / s[..., None]).clamp(0, float(steps)).long().flatten(-2)
+    per = 32 // bits
+    words = (q.unflatten(-1, (-1, per)) << (torch.arange(per) * bits)).sum(-1)
+    words = torch.where(words >= 2 ** 31, words - 2 ** 32, words).to(torch.int32)
+    return words, s.to(t), b.to(t)
+
+
 def values(codes, scales, biases, gs, bits):
     """s * q + b of packed rows [..., words] in 64 bits."""
     per = 32 // bits

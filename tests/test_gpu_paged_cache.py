@@ -1,6 +1,6 @@
 """The operators over a paged cache in 16, 8 or 4 bits against plain forms in 64 bits
 (paged_util): per-head norms with the rotation and the append, the quantised append
-bit for bit against quantize(), the read-back, and attention of decode steps, prompt
+bit for bit against its rule, the read-back, and attention of decode steps, prompt
 chunks and drafted trees, at the lengths, pages and masks where a kernel can go wrong."""
 import itertools
 import math
@@ -88,10 +88,11 @@ def test_append_norms(t, hq, hkv, hd, T, qn, kn):
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hd,gs", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
 @pytest.mark.parametrize("T,norms", [(1, True), (37, False), (600, True)])
-def test_append_quantised_is_quantize_of_the_rows(t, bits, hd, gs, T, norms):
-    """Codes, scales and biases of the written rows are quantize()'s of the rows the 16-bit
-    form writes, bit for bit (constant groups, zero rows and outliers among them); the
-    queries are the same, and rows without a slot keep what they held."""
+def test_append_quantised_is_the_rule_on_the_rows(t, bits, hd, gs, T, norms):
+    """Codes, scales and biases of the written rows are the rule's on the rows the 16-bit
+    form writes, bit for bit (constant groups, zero rows, outliers and groups whose ends
+    have one magnitude among them); the queries are the same, and rows without a slot keep
+    what they held."""
     hq, hkv, page = 7, 1 if T == 37 else 3, 8
     hq = hq * hkv
     g = _gen(T + gs + bits)
@@ -101,6 +102,10 @@ def test_append_quantised_is_quantize_of_the_rows(t, bits, hd, gs, T, norms):
     if T > 3:
         qkv[1] = 2.5
         qkv[2, ::17] *= 300.0
+    if T > 30:   # values and keys whose groups reach as far up as down
+        qkv[20:30, 0::gs] = 3.25
+        qkv[20:30, 5::gs] = -3.25
+        qkv[20:30] = qkv[20:30].clamp(-3.25, 3.25)
     qkv = qkv.to(t)
     w = (1 + 0.3 * _randn(g, hd)).to(t) if norms else None
     positions = torch.randint(0, 5000, (T,), device="cuda", generator=g, dtype=torch.int32)
@@ -124,11 +129,13 @@ def test_append_quantised_is_quantize_of_the_rows(t, bits, hd, gs, T, norms):
     rest = torch.ones(pages * page, dtype=torch.bool, device="cuda")
     rest[live] = False
     for c16, c in zip(plain, (kq, vq)):
-        ref = quantized_pool(c16, gs, bits)
-        for name in ("codes", "scales", "biases"):
-            a, b = getattr(c, name).flatten(0, 1), getattr(ref, name).flatten(0, 1)
-            a, b = (x.view(torch.int32) if name == "codes" else x.view(torch.int16) for x in (a, b))
-            assert torch.equal(a[live], b[live]), name
+        rows = c16.flatten(0, 1)[live]
+        words, scales, biases = (x.cuda() for x in P.quantized(rows, gs, bits))
+        got = [c.codes.view(torch.int32), c.scales.view(torch.int16), c.biases.view(torch.int16)]
+        got = [x.flatten(0, 1)[live] for x in got]
+        assert torch.equal(got[0], words)
+        assert torch.equal(got[1], scales.view(torch.int16))
+        assert torch.equal(got[2], biases.view(torch.int16))
         assert bool((c.scales.flatten(0, 1)[rest] == 3).all())
         assert bool((c.biases.flatten(0, 1)[rest] == -2).all())
         assert bool((c.codes.view(torch.int32).flatten(0, 1)[rest] == 0x5a5a5a5a).all())
