@@ -1,5 +1,6 @@
 // extern "C" entry points of the operators over a paged cache in 16, 8 or 4 bits (declared
 // in include/mlxq_b200.h): host-side validation, then the launches.
+#include <cmath>
 #include <cstdio>
 
 #include "../../include/mlxq_b200.h"
@@ -84,8 +85,10 @@ int mlxq_norm_rope_kv_append(const mlxq_kv_cache* cache, const void* qkv, int64_
     if (tokens < 0 || tokens > kIntMax ||
         ld < (n_q_heads + 2 * static_cast<int64_t>(c.Hkv)) * c.hd || ld % 8 || ld > kIntMax)
         return fail(MLXQ_ERR_SHAPE, what, "ld must hold q, k and v (a multiple of 8)");
-    if (!(rope_base > 1.0f)) return fail(MLXQ_ERR_SHAPE, what, "rope_base must be > 1");
-    if (!(eps >= 0.0f)) return fail(MLXQ_ERR_SHAPE, what, "eps must be >= 0");
+    if (!(rope_base > 1.0f) || !std::isfinite(rope_base))
+        return fail(MLXQ_ERR_SHAPE, what, "rope_base must be > 1 and finite");
+    if (!(eps >= 0.0f) || !std::isfinite(eps))
+        return fail(MLXQ_ERR_SHAPE, what, "eps must be >= 0 and finite");
     if (tokens == 0) return MLXQ_OK;
     if (!qkv || !q_out || !positions || !slots) return fail(MLXQ_ERR_NULL, what, "NULL pointer");
     if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(q_norm, 16) || !aligned(k_norm, 16))
@@ -148,10 +151,16 @@ int mlxq_paged_attention_rows(const mlxq_kv_cache* cache, const void* q, const i
         return fail(MLXQ_ERR_SHAPE, what, "max_kv_len must be in [0, max_blocks * page_size]");
     if (tree_mask && max_q_len > 64)
         return fail(MLXQ_ERR_SHAPE, what, "a tree has at most 64 tokens");
-    if (total == 0 || batch == 0 || max_q_len == 0) return MLXQ_OK;
-    if (!q || !block_table || !kv_lens || !out) return fail(MLXQ_ERR_NULL, what, "NULL pointer");
+    if (!std::isfinite(scale)) return fail(MLXQ_ERR_SHAPE, what, "scale must be finite");
+    if (total == 0) return MLXQ_OK;
+    if (!out) return fail(MLXQ_ERR_NULL, what, "NULL pointer");
     if (!aligned(q, 16) || !aligned(out, 16))
         return fail(MLXQ_ERR_ALIGN, what, "q and out must be 16-byte aligned");
+    if (batch == 0 || max_q_len == 0)  // every row is behind the last sequence
+        return done(cudaMemsetAsync(out, 0, static_cast<size_t>(total) * n_q_heads * c.hd * 2,
+                                    static_cast<cudaStream_t>(stream)),
+                    what);
+    if (!q || !block_table || !kv_lens) return fail(MLXQ_ERR_NULL, what, "NULL pointer");
     mlxq::RowsArgs a;
     a.q = q;
     a.out = out;

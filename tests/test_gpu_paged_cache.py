@@ -359,6 +359,42 @@ def test_rows_behind_the_last_sequence(how, bits):
     assert torch.equal(got[:37], want) and not bool(got[37:].any())
 
 
+def test_nothing_but_padding():
+    """No sequence, or none with a token: every row is behind the last and comes out zero."""
+    p = _problem(7, BF, 4, 64, 7, 1, 128, 16, [30], [3], tree=True)
+    m = torch.zeros(3, dtype=torch.int64, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out = A.paged_attention_tree(p["q"], _i32([0]), 4, p["kc"], p["vc"], none.reshape(0, 2), none,
+                                 0, m, 0.1)
+    assert out.shape == p["q"].shape and not bool(out.any())
+    bt = _i32(p["table"]["rows"])
+    for cu, max_q in (([0, 0], 0), ([0, 0], 4)):
+        out = A.paged_attention_tree(p["q"], _i32(cu), max_q, p["kc"], p["vc"], bt, _i32([30]), 30,
+                                     m, 0.1)
+        assert not bool(out.any())
+    out = A.paged_attention_decode(p["q"][:0], p["kc"], p["vc"], none.reshape(0, 2), none, 0, 0.1)
+    assert out.shape == (0, 7, 128)
+    # sequences without a key, and no key anywhere
+    out = A.paged_attention_tree(p["q"], _i32([0, 3]), 3, p["kc"], p["vc"], bt, _i32([0]), 0, m, 0.1)
+    assert not bool(out.any())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_sequences_in_groups(bits):
+    """More expanded keys than are held at once: the sequences are taken group by group."""
+    news, lens = [20, 0, 5, 33, 1], [4000, 3, 2500, 33, 700]
+    p = _problem(13, BF, bits, 64, 8, 2, 128, 16, lens, news)
+    bound = 300_000          # keys a sequence could have: 614 MB of them, so two groups and more
+    width = bound // 16
+    rows = [r + [0] * (width - len(r)) for r in p["table"]["rows"]]
+    p["table"] = dict(p["table"], rows=rows)
+    got = (_run(p, "prefill") if bits != 16 else
+           A.paged_attention_tree(p["q"], _i32(p["cu"]), 33, p["kc"], p["vc"], _i32(rows),
+                                  _i32(lens), bound,
+                                  A.tree_masks([list(range(-1, n - 1)) for n in news]), p["scale"]))
+    _check(p, got)
+
+
 def test_lengths_past_their_bounds_stay_in_bounds():
     """Device-side lengths and offsets that break the contract are cut to it."""
     p = _problem(8, BF, 4, 64, 8, 2, 64, 16, [50, 20], [4, 3], tree=True)

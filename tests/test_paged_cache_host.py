@@ -33,10 +33,10 @@ def append(c, ld=36 * 128, tokens=1, heads=28, base=1e4, eps=1e-6, qkv=FAKE, qn=
 
 
 def rows(c, cu=FAKE, total=5, max_q=4, blocks=4, max_kv=64, mask=FAKE, batch=2, heads=28, q=FAKE,
-         ws=None, nbytes=0):
+         ws=None, nbytes=0, scale=0.1, out=FAKE):
     return _lib.load().mlxq_paged_attention_rows(c, q, cu, total, max_q, FAKE, blocks, FAKE,
-                                                 max_kv, mask, FAKE, batch, heads, 0.1, ws, nbytes,
-                                                 None)
+                                                 max_kv, mask, out, batch, heads, scale, ws,
+                                                 nbytes, None)
 
 
 @pytest.mark.parametrize("kw,code", BAD_CACHES)
@@ -58,6 +58,8 @@ def test_append_is_checked():
     assert append(c, base=1.0) == _lib.ERR_SHAPE
     assert append(c, eps=-1e-6) == _lib.ERR_SHAPE
     assert append(c, eps=float("nan")) == _lib.ERR_SHAPE
+    assert append(c, eps=float("inf")) == _lib.ERR_SHAPE
+    assert append(c, base=float("inf")) == _lib.ERR_SHAPE
     assert append(c, qkv=None) == _lib.ERR_NULL
     assert append(c, qkv=FAKE + 8) == _lib.ERR_ALIGN
     assert append(c, qn=FAKE + 2) == _lib.ERR_ALIGN
@@ -88,7 +90,13 @@ def test_rows_are_checked():
     assert need > 0
     assert rows(c, ws=0x10000, nbytes=need - 1) == _lib.ERR_WORKSPACE
     assert rows(c, ws=0x10010, nbytes=need) == _lib.ERR_ALIGN
-    assert rows(c, total=0) == _lib.OK and rows(c, batch=0) == _lib.OK
+    assert rows(c, total=0) == _lib.OK
+    for bad in ("nan", "inf", "-inf"):
+        assert rows(c, scale=float(bad)) == _lib.ERR_SHAPE
+    assert rows(c, out=None) == _lib.ERR_NULL and rows(c, batch=0, out=None) == _lib.ERR_NULL
+    # more units of work than 31 bits count
+    assert rows(c, total=1 << 24, max_q=1 << 24, mask=None, batch=65535, blocks=1 << 20,
+                max_kv=1 << 24) == _lib.ERR_SHAPE
 
 
 def test_struct_layout():
