@@ -7,20 +7,28 @@
 //   s = scale * q . k over the visible keys, p = exp(s - m), out = sum p v / sum p
 //
 // Rows: sequence b has R = n * G query rows per kv head (its n new tokens times the G query
-// heads that share the head). They are taken in chunks of ROWS; the chunk's keys in tiles
-// of 64. The tiles of all (sequence, kv head, chunk) items form one sequence of units that
-// the CTAs share out evenly, whatever the lengths: a CTA's share is a contiguous run that
-// may end one item and begin another. A part of an item goes to a workspace slot of its
-// CTA, and attn_combine_kernel joins the parts in order of keys.
+// heads that share the head). This file's kernel takes up to eight of them (a decode step's
+// heads) or sixteen (of a quantised cache); more are tcgen05's M rows (paged_attn_tc.cu).
+// The rows' keys are taken in tiles of 128, a warp 32 of them, and the tiles of all sequences
+// form one sequence of units that the CTAs share out evenly, whatever the lengths
+// (rows_units.cuh). A part of an item goes to a workspace slot of its CTA, and
+// attn_combine_kernel joins the parts in order of keys.
 //
 // Keys are the M rows of the m16n8k16 products and query rows the N columns, so eight rows
-// (a decode step's heads) fill a tile without padding:
+// fill a tile without padding:
 //   S^T = K Q^T    A = 16 keys x 16 dims, straight from global memory: a lane's dims are
 //                  contiguous in its key's row, and q is permuted to match once
 //   O^T = V^T P^T  A = 16 dims x 16 keys, pairs of keys joined by byte permutes; P^T is S^T
 //                  rounded to T and transposed in registers (movmatrix)
 // so packed codes go from their load through registers into the product; shared memory
-// holds only the four warps' results at the end of an item.
+// holds only the four warps' results at the end of an item. Rows are loaded into registers a
+// tile ahead, page ids two.
+//
+// Over 16 bits the bytes bound it; over 4 bits the issue slots do: about 250 of the 450
+// instructions a warp takes for sixteen keys unpack codes and scale them, two issue a cycle
+// and SM. 32 sequences of 512 to 16384 4-bit keys, 8 kv heads of 128 (196 MB): 80 us, 2.5 TB/s;
+// 8-bit codes of 32 sequences of 8192 (558 MB): 100 us. Taking fewer or more CTAs to an SM,
+// shorter runs (94 to 115 us), or dequantising through shared memory were slower.
 #include "common.cuh"
 #include "kv_dequant.cuh"
 #include "overlap.cuh"

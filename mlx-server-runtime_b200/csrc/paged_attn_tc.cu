@@ -630,7 +630,8 @@ size_t tc_smem(int hd) {  // Q, two tiles each of K and V, the epilogue's 8 KB, 
     return (rt::ROWS + 4 * static_cast<size_t>(rt::KT)) * hd * 2 + 8192 + 1024;
 }
 
-int rows_per_seq(const RowsArgs& a) { return (a.max_kv + rt::KT - 1) / rt::KT * rt::KT; }
+// (a tile at least, so that a tensor map of a call without keys has rows)
+int rows_per_seq(const RowsArgs& a) { return ((a.max_kv > 0 ? a.max_kv : 1) + rt::KT - 1) / rt::KT * rt::KT; }
 
 }  // namespace
 
@@ -645,7 +646,6 @@ cudaError_t launch_rows_tc(ra::Params& p, void* expanded, bool overlap, cudaStre
     const void *k = c.k, *v = c.v;
     if (c.bits != 16) {
         int rps = rows_per_seq(p.a);
-        if (rps == 0) rps = rt::KT;
         const size_t each = static_cast<size_t>(p.a.batch) * rps * c.Hkv * c.hd * 2;
         void *ko = expanded, *vo = static_cast<char*>(expanded) + each;
         const int cpr = c.Hkv * c.hd / 8, x = cpr < 256 ? cpr : 256;
