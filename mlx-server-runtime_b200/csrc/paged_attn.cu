@@ -24,11 +24,14 @@
 // holds only the four warps' results at the end of an item. Rows are loaded into registers a
 // tile ahead, page ids two.
 //
-// Over 16 bits the bytes bound it; over 4 bits the issue slots do: about 250 of the 450
-// instructions a warp takes for sixteen keys unpack codes and scale them, two issue a cycle
-// and SM. 32 sequences of 512 to 16384 4-bit keys, 8 kv heads of 128 (196 MB): 80 us, 2.5 TB/s;
-// 8-bit codes of 32 sequences of 8192 (558 MB): 100 us. Taking fewer or more CTAs to an SM,
-// shorter runs (94 to 115 us), or dequantising through shared memory were slower.
+// What bounds it is how rows arrive: 32 sequences of up to 16384 4-bit keys (4 kv heads of 128,
+// 196 MB, 16384 down to 4500 keys) take 80 us, 2.4 TB/s, of which 15 do not depend on the
+// lengths; with the loads left out they take 47, with the unpacking left out 74, and with
+// keys that fit L2 the rate is the same. Sixteen-key pages of one head are 64-byte pieces, and
+// a head's scales a quarter of their sectors. 8-bit codes of the same heads move 2.9 TB/s,
+// 16-bit rows 4.2. Shorter runs (94 to 115 us) were slower, as were four heads' warps in one
+// CTA, which share those sectors but join four times the parts (74 us here, but 34 for 23 with
+// 64 sequences of 1000 keys and 89 for 82 over 16 bits).
 #include "common.cuh"
 #include "kv_dequant.cuh"
 #include "overlap.cuh"
