@@ -314,7 +314,8 @@ def paged_attention_tree(q: torch.Tensor, cu_q: torch.Tensor, max_q_len: int, k_
     kv_lens[b] <= max_kv_len cached ones (slots in row order, whatever the tokens' depths
     and positions). Every token sees the keys before those n, and of the n token j where
     bit j of its word in tree_mask [total] (int64) is set: see tree_masks. A row that sees
-    nothing is zero, and so are rows behind cu_q[-1]. Caches of 16 bits or QuantizedKV."""
+    nothing is zero, and so are rows behind cu_q[-1]. A value of the n new tokens that is not
+    finite reaches the rows that do not see it as well. Caches of 16 bits or QuantizedKV."""
     if tree_mask is None:
         raise ValueError("paged_attention_tree needs a tree_mask")
     return _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, max_kv_len,

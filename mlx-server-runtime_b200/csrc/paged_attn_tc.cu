@@ -451,7 +451,9 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
                         m4[x / 2 & 3] = fmaxf(m4[x / 2 & 3], fmaxf(__uint_as_float(v[x / 32][x % 32]),
                                                                    __uint_as_float(v[x / 32][x % 32 + 1])));
                     const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
-                    if (__any_sync(0xffffffffu, mx - m > 8.f)) {
+                    // (rows that are not there hold anything: they have no say in when the others
+                    // rescale, or results would change from call to call by a rounding)
+                    if (__any_sync(0xffffffffu, active && mx - m > 8.f)) {
                         const float mn = fmaxf(m, mx);
                         const float f = mn == -INFINITY ? 1.f : exp2f(m - mn);
                         m = mn;

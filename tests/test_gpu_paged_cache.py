@@ -375,7 +375,8 @@ def test_nothing_but_padding():
     out = A.paged_attention_decode(p["q"][:0], p["kc"], p["vc"], none.reshape(0, 2), none, 0, 0.1)
     assert out.shape == (0, 7, 128)
     # sequences without a key, and no key anywhere
-    out = A.paged_attention_tree(p["q"], _i32([0, 3]), 3, p["kc"], p["vc"], bt, _i32([0]), 0, m, 0.1)
+    out = A.paged_attention_tree(p["q"], _i32([0, 3]), 3, p["kc"], p["vc"], bt, _i32([0]), 0, m,
+                                 0.1)
     assert not bool(out.any())
 
 
@@ -483,6 +484,93 @@ def test_streams_and_graphs():
             assert torch.equal(o, w)
 
 
+@pytest.mark.parametrize("bits,how", [(4, "tree"), (16, "tree"), (8, "prefill")])
+def test_many_rows_at_once_and_in_graphs(bits, how):
+    """The calls of several launches and a large workspace: two of them at once on two
+    streams, eager and as captured graphs, give what each gives alone."""
+    ps = [_problem(40 + i, BF, bits, 64, 28, 4, 128, 16, [1900 - 300 * i, 77, 640], [31, 9 + i, 64],
+                   tree=how == "tree") for i in range(2)]
+    devs = [[_i32(p["table"]["rows"]), _i32(p["lens"]), _i32(p["cu"]),
+             torch.tensor(p["masks"] or [0], dtype=torch.int64, device="cuda")] for p in ps]
+
+    def call(p, d):
+        bt, lens, cu, m = d
+        if how == "tree":
+            return A.paged_attention_tree(p["q"], cu, 64, p["kc"], p["vc"], bt, lens,
+                                          max(p["lens"]), m, p["scale"])
+        return A.paged_attention_prefill(p["q"], cu, 64, p["kc"], p["vc"], bt, lens, p["scale"])
+
+    want = [call(p, d) for p, d in zip(ps, devs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ps]
+    got = []
+    for _ in range(5):
+        for st, p, d in zip(streams, ps, devs):
+            with torch.cuda.stream(st):
+                got.append(call(p, d))
+    torch.cuda.synchronize()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 2])
+    graphs, outs = [], []
+    for st, p, d in zip(streams, ps, devs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            outs.append(call(p, d))
+        graphs.append(g)
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_overlapped_launches(bits):
+    """With launch overlap every launch waits for what it reads and for what it writes over:
+    steps that append, attend (one row, a tree) and read back on the rows of the step before
+    give what they give without."""
+    hq, hkv, hd, page, n, steps = 28, 4, 128, 16, 24, 8
+    g = _gen(51)
+    qkv = _randn(g, steps, n, (hq + 2 * hkv) * hd).to(BF)
+    w = (1 + 0.2 * _randn(g, hd)).to(BF)
+    masks = A.tree_masks([[-1] + [i // 2 for i in range(n - 1)]])
+
+    def run():
+        cache = A.PagedKVCache(1, hkv, hd, 64, page, bits=bits)
+        k, v = cache.keys[0], cache.values[0]
+        bt = cache.allocate([1000], generator=torch.Generator().manual_seed(3))
+        slots = cache.slots(bt, [range(1000)])
+        args = []
+        for i in range(steps):  # (every step's tokens lie over half of the last one's)
+            at = 600 + i * n // 2
+            args.append((_i32(list(range(at, at + n))), slots[at:at + n].contiguous(),
+                         _i32([at + n]), _i32([0, n])))
+        torch.cuda.synchronize()
+        outs = []
+        for i, (pos, sl, lens, cu) in enumerate(args):
+            q = A.rope_kv_append(qkv[i], pos, sl, k, v, hq, hkv, hd, 1e6, w, w)
+            outs.append(A.paged_attention_tree(q, cu, n, k, v, bt, lens, 1000, masks, hd ** -0.5))
+            one = _i32([0, 1])
+            outs.append(A.paged_attention_tree(q[-1:], one, 1, k, v, bt, lens, 1000, masks[:1],
+                                               hd ** -0.5))
+            outs += A.kv_cache_read(k, v, sl)
+        torch.cuda.synchronize()
+        return outs
+
+    want = run()
+    for _ in range(3):
+        with mxq.launch_overlap(True):
+            got = run()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 CFG = dict(hidden_size=896, intermediate_size=1536, num_attention_heads=7, num_key_value_heads=1,
            num_hidden_layers=2, vocab_size=640, rope_theta=1e6, qk_norm=True)
 
@@ -499,8 +587,7 @@ def _decoder(bits, launch=False, cfg=CFG, B=3, max_len=160):
 @pytest.mark.parametrize("bits", [16, 8, 4])
 def test_decoder_over_each_cache(bits):
     """Prefill and decode steps of a model with head norms over a cache of each width, and
-    the captured step replayed: the graph's tokens are the eager steps'. An 8-bit cache's
-    logits stay near the 16-bit cache's."""
+    the captured step replayed: the graph's tokens are the eager steps'."""
     lengths = [5, 37, 130]
     ids = torch.randint(0, 640, (sum(lengths),), generator=torch.Generator().manual_seed(1),
                         dtype=torch.int32)
