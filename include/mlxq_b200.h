@@ -442,8 +442,11 @@ int mlxq_kv_cache_read(const mlxq_kv_cache* cache, const int32_t* slots, int64_t
  * A row that sees no key is zero, and so are the rows of out behind cu_q[batch]. Keys on
  * a page id outside [0, num_pages) are left out. A value that is not finite reaches the
  * rows that do not see its key only where the key is one of the sequence's own new tokens.
- * n_q_heads / n_kv_heads <= 8. The workspace (mlxq_paged_attention_rows_workspace_size bytes, 256-byte aligned,
- * contents arbitrary) is used until the call's work on the stream has finished.
+ * n_q_heads / n_kv_heads <= 8; batch <= 65535, total and max_q_len < 2^25, max_kv_len < 2^30,
+ * scale finite; MLXQ_ERR_SHAPE too where kv heads x chunks of rows x tiles of keys of the whole
+ * batch, at their bounds, reach 2^31. The workspace (mlxq_paged_attention_rows_workspace_size
+ * bytes, 256-byte aligned, contents arbitrary) is used until the call's work on the stream has
+ * finished. The same call gives the same bits.
  */
 size_t mlxq_paged_attention_rows_workspace_size(const mlxq_kv_cache* cache, int64_t batch,
                                                 int64_t max_q_len, int64_t max_kv_len,

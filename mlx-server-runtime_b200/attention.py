@@ -47,8 +47,8 @@ def _p(t):
 class QuantizedKV:
     """One layer's keys or values held in 8 or 4 bits: the pool a 16-bit cache tensor
     [pages, page_size, n_kv_heads, head_dim] stands for, each head's row quantized in groups
-    of group_size and laid out as quantize() does it. codes uint32 [pages, page_size, n_kv_heads, head_dim*bits/32],
-    scales and biases [pages, page_size, n_kv_heads, head_dim/group_size] of the
+    of group_size and laid out as quantize() does it. codes uint32
+    [pages, page_size, n_kv_heads, head_dim*bits/32], scales and biases [pages, page_size, n_kv_heads, head_dim/group_size] of the
     activation dtype; a code q stands for scale * q + bias, rounded once to that dtype.
     Takes a cache tensor's place in rope_kv_append, kv_cache_read and the paged
     attention functions (keys and values of the same width)."""

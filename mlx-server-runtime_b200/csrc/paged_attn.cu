@@ -30,7 +30,7 @@
 // keys that fit L2 the rate is the same. Sixteen-key pages of one head are 64-byte pieces, and
 // a head's scales a quarter of their sectors. 8-bit codes of the same heads move 2.9 TB/s,
 // 16-bit rows 4.2. Shorter runs (94 to 115 us) were slower, as were four heads' warps in one
-// CTA, which share those sectors but join four times the parts (74 us here, but 34 for 23 with
+// CTA, which share those sectors but join four times the parts (75 us here, but 32 for 23 with
 // 64 sequences of 1000 keys and 89 for 82 over 16 bits).
 #include "common.cuh"
 #include "kv_dequant.cuh"

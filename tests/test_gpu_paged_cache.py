@@ -437,6 +437,40 @@ def test_rising_scores():
         _check(p, _run(p, how))
 
 
+@pytest.mark.parametrize("bits,rows", [(16, 5 << 20), (4, 18 << 20)])
+def test_offsets_past_32_bits(bits, rows):
+    """Rows more than 2^32 bytes into their pools give what rows at the front give."""
+    hq, hkv, hd, page, T = 8, 4, 128, 16, 200
+    g = _gen(61)
+    qkv = _randn(g, T, (hq + 2 * hkv) * hd).to(BF)
+    pos = _i32(list(range(T)))
+
+    def pool():
+        shape = (rows // page, page, hkv)
+        if bits == 16:
+            return torch.empty(*shape, hd, dtype=BF, device="cuda")
+        codes = torch.empty(*shape, hd * bits // 32, dtype=torch.int32, device="cuda")
+        assert codes.numel() * 4 > 1 << 32
+        return A.QuantizedKV(codes, *(torch.empty(*shape, hd // 64, dtype=BF, device="cuda")
+                                      for _ in range(2)), 64, bits)
+
+    k, v = pool(), pool()
+    blocks = -(-T // page)
+    outs = []
+    for first in (0, rows // page - blocks):
+        slots = _i32([first * page + i for i in range(T)])
+        bt = _i32([[first + j for j in range(blocks)]])
+        q = A.rope_kv_append(qkv, pos, slots, k, v, hq, hkv, hd, 1e6, q_norm=None,
+                             k_norm=torch.ones(hd, dtype=BF, device="cuda"))
+        outs.append([*A.kv_cache_read(k, v, slots)])
+        for n in (1, 40):  # few rows of a kv head, and many
+            m = A.tree_masks([list(range(-1, n - 1))])
+            outs[-1].append(A.paged_attention_tree(q[T - n:], _i32([0, n]), n, k, v, bt, _i32([T]),
+                                                   T, m, hd ** -0.5))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b) and bool(a.any())
+
+
 def test_same_result_every_time():
     p = _problem(11, BF, 4, 64, 28, 4, 128, 16, [3000, 50, 900], [1] * 3)
     first = _run(p, "decode")
