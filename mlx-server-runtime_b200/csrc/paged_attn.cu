@@ -51,18 +51,21 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 
+// Everything here may have been written by a kernel of the same stream that still ran when
+// this one was launched (launch overlap): ordinary loads, which the wait for that kernel
+// orders, and not the read-only path, whose data must not change while a kernel runs.
 template <int N>
 __device__ __forceinline__ void ldw(const void* at, uint32_t (&r)[N]) {
     if constexpr (N == 1) {
-        r[0] = __ldg(static_cast<const uint32_t*>(at));
+        r[0] = *static_cast<const uint32_t*>(at);
     } else if constexpr (N == 2) {
-        const uint2 v = __ldg(static_cast<const uint2*>(at));
+        const uint2 v = *static_cast<const uint2*>(at);
         r[0] = v.x;
         r[1] = v.y;
     } else {
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
-            const uint4 v = __ldg(static_cast<const uint4*>(at) + i);
+            const uint4 v = static_cast<const uint4*>(at)[i];
             r[4 * i] = v.x;
             r[4 * i + 1] = v.y;
             r[4 * i + 2] = v.z;
@@ -125,7 +128,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
         // the pool's first rows (and not used).
         auto page_id = [&](int tile) -> int {
             const int key = tile * KT + warp * 32 + lane;
-            return tile < te && key < kend ? __ldg(bt + (key >> page_shift)) : -1;
+            return tile < te && key < kend ? bt[key >> page_shift] : -1;
         };
         auto row_id = [&](int tile, int pid) -> uint32_t {
             const uint32_t in = static_cast<uint32_t>(tile * KT + warp * 32 + lane) & (c.page - 1);
@@ -151,8 +154,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
                     const int id = 32 * i + lane;
                     const size_t at = static_cast<size_t>(__shfl_sync(0xffffffffu, rows, id / NG)) * (Hkv * NG) +
                                       (g * NG + id % NG);
-                    ks[i] = __ldg(static_cast<const uint16_t*>(c.ks) + at);
-                    kb[i] = __ldg(static_cast<const uint16_t*>(c.kb) + at);
+                    ks[i] = static_cast<const uint16_t*>(c.ks)[at];
+                    kb[i] = static_cast<const uint16_t*>(c.kb)[at];
                 }
             }
         };
@@ -173,8 +176,8 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
                     const int id = 32 * i + lane;
                     const size_t at = static_cast<size_t>(__shfl_sync(0xffffffffu, rows, id / NG)) * (Hkv * NG) +
                                       (g * NG + id % NG);
-                    vs[i] = __ldg(static_cast<const uint16_t*>(c.vs) + at);
-                    vb[i] = __ldg(static_cast<const uint16_t*>(c.vb) + at);
+                    vs[i] = static_cast<const uint16_t*>(c.vs)[at];
+                    vb[i] = static_cast<const uint16_t*>(c.vb)[at];
                 }
             }
         };

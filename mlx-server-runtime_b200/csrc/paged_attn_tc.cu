@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             const int key = tile * KT + box * src.box;
             if (!loads || key >= kend) return -1;
             if (src.rows_per_seq) return w.b * src.rows_per_seq + key;
-            return __ldg(a.table + static_cast<size_t>(w.b) * a.max_blocks + (key >> page_shift));
+            return a.table[static_cast<size_t>(w.b) * a.max_blocks + (key >> page_shift)];
         };
         uint32_t j = 0, lands = 0, items = 0;
         bool more = step();
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
             // which eights of a tile's keys are on pages of the pool: looked up a tile ahead
             auto page_at = [&](int k0) -> int {
                 const int key = k0 + 8 * (lane & 7);
-                return key < kend ? __ldg(bt + (key >> page_shift)) : 0;
+                return key < kend ? bt[key >> page_shift] : 0;
             };
             int pid = page_at(w.t0 * KT);
             for (int tile = w.t0; tile < te; ++tile, ++it) {
@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
 // The values of every sequence's keys, from the first to the end of its last tile (zeros
 // behind the last key and for pages outside the pool): block (tile of 64 keys, sequence,
 // keys or values), thread = (eight values of a row, row), so that a warp reads and writes
-// one span; eight rows in flight.
+// one span; eight rows in flight. (Ordinary loads: see ldw in paged_attn.cu.)
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
     kv_expand_kernel(const KvCache c, const RowsArgs a, int rows_per_seq, T* __restrict__ k_out,
@@ -567,21 +567,21 @@ __global__ void __launch_bounds__(256)
             for (int j = 0; j < AHEAD; ++j) {
                 const int r = r0 + j * blockDim.y, key = k0 + r;
                 int pid = -1;
-                if (r < rt::KT && key < L) pid = __ldg(bt + (key >> page_shift));
+                if (r < rt::KT && key < L) pid = bt[key >> page_shift];
                 const bool in = pid >= 0 && pid < c.pages;
                 there |= in ? 1u << j : 0u;
                 // (a row that is not there is read from the pool's first, and not used)
                 const uint32_t row = in ? (static_cast<uint32_t>(pid) << page_shift) + (key & (c.page - 1)) : 0u;
                 const uint32_t* at = codes + static_cast<size_t>(row) * (cpr * (BITS / 4));
                 if constexpr (BITS == 8) {
-                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(at));
+                    const uint2 v = *reinterpret_cast<const uint2*>(at);
                     raw[j][0] = v.x;
                     raw[j][1] = v.y;
                 } else {
-                    raw[j][0] = __ldg(at);
+                    raw[j][0] = *at;
                 }
-                s[j] = __ldg(sp + static_cast<size_t>(row) * gpr);
-                z[j] = __ldg(bp + static_cast<size_t>(row) * gpr);
+                s[j] = sp[static_cast<size_t>(row) * gpr];
+                z[j] = bp[static_cast<size_t>(row) * gpr];
             }
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {

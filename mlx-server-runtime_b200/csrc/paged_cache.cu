@@ -265,8 +265,8 @@ cudaError_t launch_norm_rope_append(const KvCache& c, const void* qkv, long long
 // the keys (blockIdx.y 0) or the values (1). Slots outside the pool give zeros.
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256)
-    cache_read_kernel(const KvCache c, const int32_t* __restrict__ slots, long long n8,
-                      T* __restrict__ k_out, T* __restrict__ v_out) {
+    cache_read_kernel(const KvCache c, const int32_t* slots, long long n8,
+                      T* k_out, T* v_out) {
     pdl_launch_dependents();
     pdl_wait();
     const bool is_v = blockIdx.y != 0;
