@@ -414,8 +414,10 @@ typedef struct mlxq_kv_cache {
  * (models/qwen3.py of the reference). Norm and rotation are one 32-bit
  * computation rounded once; the angle is reduced in 64 bits. With bits 8 or 4 the rounded
  * rows are quantized by mlxq_quantize's rule, but for a group's range, which is multiplied by
- * the 32-bit reciprocal of its steps (15 or 255) rather than divided by them. Slots outside
- * [0, num_pages * page_size) are skipped; two tokens of one call must not share a slot.
+ * the 32-bit reciprocal of its steps (15 or 255) rather than divided by them, and for a group
+ * that holds a NaN or an infinity, which stands for NaN as a whole (mlxq_quantize passes over a
+ * NaN). Slots outside [0, num_pages * page_size) are skipped; two tokens of one call must not
+ * share a slot.
  */
 int mlxq_norm_rope_kv_append(const mlxq_kv_cache* cache, const void* qkv, int64_t ld, void* q_out,
                              const void* q_norm, const void* k_norm, float eps,

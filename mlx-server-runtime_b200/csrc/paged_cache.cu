@@ -33,6 +33,19 @@ struct AppendArgs {
 
 __device__ __forceinline__ uint2 ld8(const void* p) { return *reinterpret_cast<const uint2*>(p); }
 
+// Minimum and maximum that are no number where one of the two is none (fminf and fmaxf
+// return the other).
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 }  // namespace
 
 // One warp takes `rounds` groups of 32 / LPH heads of a token; the LPH = HD / 8 lanes of a
@@ -45,8 +58,10 @@ __device__ __forceinline__ uint2 ld8(const void* p) { return *reinterpret_cast<c
 // 32-bit sine and cosine of the rest, one pair to a thread and through shared memory to the
 // CTA's warps: worked out by every warp for itself, they were a third of the instructions,
 // which is what bounds a prompt's append. In a quantised cache the row rounded to T is
-// quantised by quantize()'s rule (see quant_group): a group's least and largest value by shuffles over its
-// lanes, four codes per lane and half.
+// quantised by quantize()'s rule (see quant_group): a group's least and largest value by
+// shuffles over its lanes, four codes per lane and half. A NaN in a group makes both of them
+// one, an infinity the range, and so the group's scale: it then stands for NaN, as its row does
+// in 16 bits, and not for a number that nothing computed.
 template <typename T, int HD, int BITS>
 __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int LPH = HD / 8, HPW = 32 / LPH, HALF = HD / 2;
@@ -142,22 +157,22 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
             float mn[2] = {INFINITY, INFINITY}, mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                mn[0] = fminf(mn[0], p[j]); mx[0] = fmaxf(mx[0], p[j]);
-                mn[1] = fminf(mn[1], q[j]); mx[1] = fmaxf(mx[1], q[j]);
+                mn[0] = min_nan(mn[0], p[j]); mx[0] = max_nan(mx[0], p[j]);
+                mn[1] = min_nan(mn[1], q[j]); mx[1] = max_nan(mx[1], q[j]);
             }
             const bool whole = c.gs == HD;  // one group: both halves
             if (whole) {
-                mn[0] = mn[1] = fminf(mn[0], mn[1]);
-                mx[0] = mx[1] = fmaxf(mx[0], mx[1]);
+                mn[0] = mn[1] = min_nan(mn[0], mn[1]);
+                mx[0] = mx[1] = max_nan(mx[0], mx[1]);
             }
             const int seg = min(LPH, c.gs / 4);  // lanes of a group
             // even lanes go on with the lower half's group, odd lanes with the upper half's
             const int side = li & 1;
-            float lo_s = fminf(mn[side], __shfl_xor_sync(0xffffffffu, mn[side ^ 1], 1));
-            float hi_s = fmaxf(mx[side], __shfl_xor_sync(0xffffffffu, mx[side ^ 1], 1));
+            float lo_s = min_nan(mn[side], __shfl_xor_sync(0xffffffffu, mn[side ^ 1], 1));
+            float hi_s = max_nan(mx[side], __shfl_xor_sync(0xffffffffu, mx[side ^ 1], 1));
             for (int o = seg >> 1; o > 1; o >>= 1) {
-                lo_s = fminf(lo_s, __shfl_xor_sync(0xffffffffu, lo_s, o));
-                hi_s = fmaxf(hi_s, __shfl_xor_sync(0xffffffffu, hi_s, o));
+                lo_s = min_nan(lo_s, __shfl_xor_sync(0xffffffffu, lo_s, o));
+                hi_s = max_nan(hi_s, __shfl_xor_sync(0xffffffffu, hi_s, o));
             }
             constexpr float n_bins = static_cast<float>((1 << BITS) - 1);
             float sc[2], bi[2], rc[2];

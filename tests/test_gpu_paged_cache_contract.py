@@ -1,0 +1,90 @@
+"""The paged-cache operators where the other tests of them do not go: values that are not
+finite."""
+import math
+
+import pytest
+import torch
+
+from mlx_server_runtime_b200 import attention as A
+
+import test_gpu_paged_cache as base
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+# ---------------------------------------------------------------------------- not finite
+
+@pytest.mark.parametrize("t", [BF, HF])
+@pytest.mark.parametrize("bits,hd,gs", [(4, 64, 32), (4, 128, 64), (8, 64, 64), (8, 128, 128),
+                                        (8, 128, 32), (4, 128, 128)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("norms", [True, False])
+def test_append_of_values_that_are_not_finite(t, bits, hd, gs, value, norms):
+    """A group that holds a NaN or an infinity reads back as NaN, all of it, and every other
+    group as it does without."""
+    hq, hkv, T, page = 4, 2, 6, 8
+    g = base._gen(bits + hd + gs)
+    clean = base._randn(g, T, (hq + 2 * hkv) * hd).to(t)
+    qkv = clean.clone()
+    k_at, v_at = hq * hd, (hq + hkv) * hd
+    hit = [(1, 0, 3), (2, 1, hd - 1), (4, 1, hd // 2)]     # token, head, element
+    for tok, h, e in hit:
+        qkv[tok, k_at + h * hd + e] = value
+        qkv[tok, v_at + h * hd + e] = value
+    w = torch.ones(hd, dtype=t, device="cuda") if norms else None
+    ids = base._i32(list(range(T)))
+    outs = []
+    for x in (clean, qkv):
+        kc, vc = (A.QuantizedKV.zeros(2, page, hkv, hd, gs, bits, t) for _ in range(2))
+        A.rope_kv_append(x, ids + 3, ids, kc, vc, hq, hkv, hd, 1e4, q_norm=w, k_norm=w)
+        outs.append(A.kv_cache_read(kc, vc, ids))
+    lost_k = torch.zeros(T, hkv, hd, dtype=torch.bool, device="cuda")
+    lost_v = lost_k.clone()
+    for tok, h, e in hit:
+        lost_v[tok, h, e // gs * gs:(e // gs + 1) * gs] = True
+        if norms:          # (the mean of squares is none of the head's values' any more)
+            lost_k[tok, h] = True
+        else:              # the element and the one it is rotated with
+            for x in (e, (e + hd // 2) % hd):
+                lost_k[tok, h, x // gs * gs:(x // gs + 1) * gs] = True
+    if norms and math.isinf(value):
+        # an infinite mean of squares makes zeros of the finite elements and a NaN of the
+        # infinite one, so only the groups of its pair are lost
+        lost_k[:] = False
+        for tok, h, e in hit:
+            for x in (e, (e + hd // 2) % hd):
+                lost_k[tok, h, x // gs * gs:(x // gs + 1) * gs] = True
+    for want, got, lost in zip(outs[0], outs[1], (lost_k, lost_v)):
+        assert bool(torch.isnan(got[lost]).all())
+        same = ~lost
+        if lost is lost_k and norms and math.isinf(value):
+            for tok, h, _ in hit:      # (the rest of those heads is zeros: checked apart)
+                rest = got[tok, h][~lost[tok, h]]
+                assert not bool(rest.any())
+                same[tok, h] = False
+        assert torch.equal(got[same], want[same])
+
+
+@pytest.mark.parametrize("how,bits,hd", [("decode", 4, 128), ("decode", 8, 64), ("tree", 16, 128),
+                                         ("tree", 16, 64), ("tree", 4, 128), ("prefill", 8, 64)])
+@pytest.mark.parametrize("side", ["k", "v"])
+def test_a_key_or_value_that_is_none_shows(how, bits, hd, side):
+    """A NaN in a key every row of its sequence sees makes those rows of the kv head NaN, one
+    in a value the elements it stands for; other heads and sequences keep their bits."""
+    hq, hkv, gs = 8, 2, 32
+    news = [1] * 3 if how == "decode" else [20, 5, 30]
+    p = base._problem(71, BF, bits, gs, hq, hkv, hd, 16, [150, 40, 300], news, tree=how == "tree")
+    want = base._run(p, how)
+    at = p["table"]["rows"][2][130 // 16] * 16 + 130 % 16      # key 130 of the last sequence
+    c = p[side + "c"]
+    (c if bits == 16 else c.scales).flatten(0, 1)[at, 1, 0] = math.nan
+    got = base._run(p, how)
+    lost = torch.zeros_like(got, dtype=torch.bool)
+    lo = p["cu"][2] if how != "decode" else 2
+    if side == "k":
+        lost[lo:, hq // 2:] = True
+    else:
+        lost[lo:, hq // 2:, :1 if bits == 16 else gs] = True
+    assert bool(torch.isnan(got[lost]).all())
+    assert torch.equal(got[~lost], want[~lost])
