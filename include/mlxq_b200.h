@@ -414,7 +414,10 @@ typedef struct mlxq_kv_cache {
  * (models/qwen3.py of the reference). Norm and rotation are one 32-bit
  * computation rounded once; the angle is reduced in 64 bits. With bits 8 or 4 the rounded
  * rows are quantized by mlxq_quantize's rule, but for a group's range, which is multiplied by
- * the 32-bit reciprocal of its steps (15 or 255) rather than divided by them, and for a group
+ * the 32-bit reciprocal of its steps (15 or 255) rather than divided by them (the group is then
+ * the same, bit for bit, but where its larger end lies half way between two codes from zero: 0.4
+ * to 0.6 % of 4-bit bf16 groups of normal data, 0.05 to 0.25 % of others, whose values may differ
+ * by a step and a half, with the rounding of their scales by up to three and a half), and for a group
  * that holds a NaN or an infinity, which stands for NaN as a whole (mlxq_quantize passes over a
  * NaN). Slots outside [0, num_pages * page_size) are skipped; two tokens of one call must not
  * share a slot.

@@ -50,6 +50,8 @@ class QuantizedKV:
     of group_size and laid out as quantize() does it. codes uint32
     [pages, page_size, n_kv_heads, head_dim*bits/32], scales and biases [pages, page_size, n_kv_heads, head_dim/group_size] of the
     activation dtype; a code q stands for scale * q + bias, rounded once to that dtype.
+    Rows that rope_kv_append writes are quantize()'s too, bit for bit, but for groups whose
+    larger end lies half way between two codes from zero (under one in a hundred).
     Takes a cache tensor's place in rope_kv_append, kv_cache_read and the paged
     attention functions (keys and values of the same width)."""
     codes: torch.Tensor

@@ -30,10 +30,16 @@ __device__ __forceinline__ uint32_t quant_code(float d, float s, float r, float 
 
 // Scale and bias of a group from its least and largest value and a first step, its range
 // over the number of steps: the end of larger magnitude is kept exactly (bias = that end,
-// scale = end / code of zero). quantize_kernel divides for the step; the cache multiplies by
-// the steps' reciprocal, a division fewer. The two can differ in the step's last bit, which
-// decides where the end lies half way between two codes from zero (ends of one magnitude, for
-// one): either neighbour then serves.
+// scale = end / code of zero). There are two rules, which differ in the step alone:
+// quantize_kernel divides the range, the cache multiplies it by the steps' reciprocal. The scale
+// is made anew from the code of zero, so groups come out the same, bit for bit, unless that code
+// differs: where the larger end lies half way between two codes from zero (to 2^-22 of it), as
+// with ends of one magnitude. The lower neighbour then spans the range and misses a value by
+// 0.54 steps of 15 at most, the upper one clips the far end by up to a step, and what the two
+// stand for differs by a step and a half, before scales are rounded to 16 bits. Of normal data,
+// 0.37 to 0.63 % of 4-bit and 0.07 to 0.25 % of 8-bit bf16 groups differ (0.05 to 0.09 % in
+// f16). In 4 bits the cache's rule took the lower one each time, and so misses values by 0.58
+// steps at most where quantize()'s misses them by 0.94 (scales rounded).
 __device__ __forceinline__ void quant_group(float lmin, float lmax, float step, float& scale,
                                             float& bias) {
     const bool mask = fabsf(lmin) > fabsf(lmax);

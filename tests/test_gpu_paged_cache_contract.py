@@ -1,12 +1,14 @@
 """The paged-cache operators where the other tests of them do not go: values that are not
-finite."""
+finite, and the cache's quantisation beside quantize()'s."""
 import math
 
 import pytest
 import torch
 
+import mlx_server_runtime_b200 as mxq
 from mlx_server_runtime_b200 import attention as A
 
+import paged_util as P
 import test_gpu_paged_cache as base
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +90,55 @@ def test_a_key_or_value_that_is_none_shows(how, bits, hd, side):
         lost[lo:, hq // 2:, :1 if bits == 16 else gs] = True
     assert bool(torch.isnan(got[lost]).all())
     assert torch.equal(got[~lost], want[~lost])
+
+
+# ---------------------------------------------------------------------------- the two rules
+
+@pytest.mark.parametrize("t", [BF, HF])
+@pytest.mark.parametrize("bits,hd,gs", [(4, 128, 64), (8, 128, 64), (4, 64, 32), (8, 128, 128)])
+def test_append_beside_quantize(t, bits, hd, gs):
+    """Values appended to a quantised cache and the same rows through quantize(). Groups
+    are the same, bit for bit, unless the larger end lies half way between two codes from
+    zero; then one rule may take one neighbour and the other the next, and what the group
+    stands for differs by a step and a half at most, with the rounding of scales and
+    values.
+
+    Half way: both steps are range / n within 3 * 2^-24 of it (the product's two roundings
+    and the reciprocal's; the quotient's one), the end over the step is rounded once more, so
+    the two differ only where a half-integer lies within 2^-22 of end * n / range, relatively.
+
+    A step and a half: with the end at m + 1/2 steps, m codes span the range (m + 1/2) / m
+    times over and miss a value by half a code, (m + 1/2) / 2m steps; m + 1 codes clip the far
+    end by n / 2(m + 1) steps. The larger end is at least n / 2 steps off, m >= (n - 1) / 2:
+    0.536 and 1 steps (n = 15). A scale is rounded to t (n codes of it), each value too."""
+    hq, hkv, T = 1, 1, 20000
+    n = 2 ** bits - 1
+    g = base._gen(bits + hd + gs)
+    qkv = base._randn(g, T, 3 * hd)
+    qkv[:200, 0::gs] = 3.25                       # ends of one magnitude
+    qkv[:200, 5::gs] = -3.25
+    qkv[:200] = qkv[:200].clamp(-3.25, 3.25)
+    qkv = qkv.to(t)
+    ids = base._i32(list(range(T)))
+    kc, vc = (A.QuantizedKV.zeros(-(-T // 16), 16, hkv, hd, gs, bits, t) for _ in range(2))
+    A.rope_kv_append(qkv, ids, ids, kc, vc, hq, hkv, hd, 1e4)
+    rows = qkv[:, 2 * hd:].contiguous()
+    w, s, b = mxq.quantize(rows, gs, bits)
+    mine = [vc.codes.flatten(0, 2)[:T], vc.scales.flatten(0, 2)[:T], vc.biases.flatten(0, 2)[:T]]
+    per = gs * bits // 32
+    same = (mine[0].view(torch.int32).unflatten(-1, (-1, per)) ==
+            w.view(torch.int32).unflatten(-1, (-1, per))).all(-1)
+    same &= (mine[1].view(torch.int16) == s.view(torch.int16))
+    same &= (mine[2].view(torch.int16) == b.view(torch.int16))
+    v = rows.double().unflatten(-1, (-1, gs))
+    hi, lo = v.amax(-1), v.amin(-1)
+    step = (hi - lo) / n
+    ends = torch.maximum(hi.abs(), lo.abs()) / step
+    off = (ends - (ends.floor() + 0.5)).abs()
+    assert bool((off <= 2.0 ** -22 * ends)[~same].all())
+    assert 0 < int((~same).sum()) < same.numel() // 50
+    va, vb = (P.values(*x, gs, bits).float().to(t).double().unflatten(-1, (-1, gs))
+              for x in (mine, (w, s, b)))
+    room = step * (1.54 + 2 * n * 1.08 * P.U[t])
+    bound = room[..., None] + P.U[t] * (va.abs() + vb.abs()) * 1.01
+    assert bool(((va - vb).abs() <= bound).all())
