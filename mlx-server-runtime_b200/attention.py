@@ -268,7 +268,8 @@ def kv_cache_read(k_cache, v_cache, slots: torch.Tensor):
 
 def _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, max_kv_len,
                     tree_mask, scale, what):
-    """mlxq_paged_attention_rows: a cache of any width, one or several rows a sequence."""
+    """mlxq_paged_attention_rows: a cache of any width, one or several rows a sequence.
+    max_kv_len None: what the block table can hold."""
     kv = _kv_struct(k_cache, v_cache)
     shape = q.shape
     if len(shape) != 3 or _DT.get(q.dtype) != kv.dtype or shape[2] != kv.head_dim:
@@ -291,7 +292,8 @@ def _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens, 
         tree_mask = tree_mask.contiguous()
     dev = _on(q, cu_q, _pool(k_cache), _pool(v_cache), block_table, kv_lens, tree_mask)
     out = torch.empty_like(q)
-    max_q_len, max_kv_len = int(max_q_len), int(max_kv_len)
+    max_q_len = int(max_q_len)
+    max_kv_len = blocks * kv.page_size if max_kv_len is None else int(max_kv_len)
     L = _lib.load()
 
     def call(st):
@@ -383,15 +385,15 @@ def paged_attention_decode(q: torch.Tensor, k_cache, v_cache,
 def paged_attention_prefill(q: torch.Tensor, cu_q: torch.Tensor, max_q_len: int,
                             k_cache, v_cache,
                             block_table: torch.Tensor, kv_lens: torch.Tensor,
-                            scale: float) -> torch.Tensor:
+                            scale: float, max_kv_len: int | None = None) -> torch.Tensor:
     """New tokens of every sequence: q [total, n_heads, head_dim], sequence b's rows
     [cu_q[b], cu_q[b+1]) at the last positions of its kv_lens[b] cached keys, causal. The
-    caches are 16-bit tensors or a pair of QuantizedKV."""
+    caches are 16-bit tensors or a pair of QuantizedKV. max_kv_len is a bound on kv_lens
+    (default: what the block table can hold): over a QuantizedKV it sizes the workspace and
+    the work, so give it where tables are wider than the sequences."""
     if isinstance(k_cache, QuantizedKV) or isinstance(v_cache, QuantizedKV):
-        page = k_cache.shape[1]
         return _rows_attention(q, cu_q, max_q_len, k_cache, v_cache, block_table, kv_lens,
-                               block_table.shape[-1] * page, None, scale,
-                               "paged_attention_prefill")
+                               max_kv_len, None, scale, "paged_attention_prefill")
     dt = _code(q, "q")
     page, hkv, hd = _cache_geometry(k_cache, v_cache, q)
     _, H, _ = q.shape
@@ -400,6 +402,8 @@ def paged_attention_prefill(q: torch.Tensor, cu_q: torch.Tensor, max_q_len: int,
     B = block_table.shape[0]
     if cu_q.shape != (B + 1,):
         raise ValueError(f"cu_q must be [{B + 1}] (one offset per sequence, then the total)")
+    if max_kv_len is not None and not 0 <= max_kv_len <= block_table.shape[1] * page:
+        raise ValueError("max_kv_len must be in [0, max_blocks * page_size]")
     out = torch.empty_like(q)
     with torch.cuda.device(q.device):
         rc = _lib.load().mlxq_paged_attention_prefill(

@@ -98,7 +98,8 @@ class Qwen2Attention(nn.Module):
                                        batch.max_kv_len, self.scale)
         else:
             a = paged_attention_prefill(q, batch.cu_q, batch.max_q_len, k_cache, v_cache,
-                                        batch.block_table, batch.kv_lens, self.scale)
+                                        batch.block_table, batch.kv_lens, self.scale,
+                                        batch.max_kv_len)
         return self.o_proj(a.reshape(a.shape[0], -1))
 
 

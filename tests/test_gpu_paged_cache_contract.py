@@ -1,12 +1,13 @@
 """The paged-cache operators where the other tests of them do not go: values that are not
-finite, and the cache's quantisation beside quantize()'s."""
+finite, the cache's quantisation beside quantize()'s, and block tables far wider than the
+sequences."""
 import math
 
 import pytest
 import torch
 
 import mlx_server_runtime_b200 as mxq
-from mlx_server_runtime_b200 import attention as A
+from mlx_server_runtime_b200 import attention as A, qwen2
 
 import paged_util as P
 import test_gpu_paged_cache as base
@@ -142,3 +143,54 @@ def test_append_beside_quantize(t, bits, hd, gs):
     room = step * (1.54 + 2 * n * 1.08 * P.U[t])
     bound = room[..., None] + P.U[t] * (va.abs() + vb.abs()) * 1.01
     assert bool(((va - vb).abs() <= bound).all())
+
+
+# ---------------------------------------------------------------------------- wide tables
+
+def _peak(call):
+    """A call's result and the most memory it held beyond what was held before."""
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = call()
+    torch.cuda.synchronize()
+    return out, torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_prefill_in_wide_tables(bits):
+    """max_kv_len sizes a chunk's work, whatever the block table could hold: the same bits
+    and the same memory in a table for 640 keys and in one for 32768."""
+    news, lens = [300, 77, 512], [512, 77, 512]
+    p = base._problem(14, BF, bits, 64, 28, 4, 128, 16, lens, news)
+    cu, kv = base._i32(p["cu"]), base._i32(lens)
+    outs = []
+    for capacity in (640, 32768):
+        bt = base._i32([r + [0] * (capacity // 16 - len(r)) for r in p["table"]["rows"]])
+        outs.append(_peak(lambda: A.paged_attention_prefill(
+            p["q"], cu, 512, p["kc"], p["vc"], bt, kv, p["scale"], max_kv_len=512)))
+    assert torch.equal(outs[0][0], outs[1][0])
+    assert outs[0][1] == outs[1][1]
+    if bits != 16:
+        base._check(p, outs[1][0])
+    for bad in (-1, 32769):
+        with pytest.raises(ValueError, match="max_kv_len"):
+            A.paged_attention_prefill(p["q"], cu, 512, p["kc"], p["vc"], bt, kv, p["scale"],
+                                      max_kv_len=bad)
+
+
+def test_decoder_prefills_in_wide_tables():
+    """The decoder gives the prompts' lengths on: its prefill takes no more memory with room
+    for 8192 tokens a sequence than with room for 256."""
+    c = qwen2.Qwen2Config(**base.CFG)
+    model = qwen2.Qwen2ForCausalLM(c, seed=3)
+    lengths = [5, 37, 130]
+    ids = torch.randint(0, 640, (sum(lengths),), generator=torch.Generator().manual_seed(1),
+                        dtype=torch.int32)
+    got = []
+    for max_len in (256, 256, 8192):       # (the first sets workspaces up)
+        cache = A.PagedKVCache(2, 1, 128, num_pages=3 * max_len // 16, bits=8)
+        dec = qwen2.GreedyDecoder(model, cache, 3, max_len=max_len)
+        got.append(_peak(lambda: dec.prefill(ids, lengths)))
+    assert torch.equal(got[1][0], got[2][0])
+    assert abs(got[1][1] - got[2][1]) < 1 << 20

@@ -3,8 +3,9 @@ import os
 import re
 
 import pytest
+import torch
 
-from mlx_server_runtime_b200 import _lib
+from mlx_server_runtime_b200 import _lib, attention as A
 
 CSRC = os.path.join(os.path.dirname(_lib.__file__), "csrc")
 
@@ -26,3 +27,26 @@ def test_no_read_only_loads(name):
     s = source(name)
     assert not re.search(r"__ldg\b|\bld\.global(\.\w+)*\.nc\b", s)
     assert not re.search(r"\bconst\b[^;,(){}]*\*\s*__restrict__", s)
+
+
+def test_prefill_bounds_its_lengths():
+    """max_kv_len is at most what the block table holds (two pages of 16 here)."""
+    c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    i32 = torch.zeros(4, 2, dtype=torch.int32)
+    for bad in (-1, 33):
+        with pytest.raises(ValueError, match="max_kv_len"):
+            A.paged_attention_prefill(q, i32[:, 0], 4, c, c, i32[:3], i32[:3, 0], 0.1,
+                                      max_kv_len=bad)
+
+
+@pytest.mark.parametrize("batch,max_kv,hkv,hd", [(64, 32768, 4, 128), (3, 1 << 20, 8, 128),
+                                                 (500, 600, 2, 64), (1, 100, 1, 64)])
+def test_expansion_workspace_is_bounded(batch, max_kv, hkv, hd):
+    """1 GiB of expanded rows, or one sequence's where they are more; beside them the parts of
+    at most two CTAs an SM (two slots of 128 rows each) and 1 KiB a sequence to align."""
+    c = _lib.KVCache(*[0x1000] * 6, 8, 16, hkv, hd, 4, 64, _lib.BF16)
+    need = _lib.load().mlxq_paged_attention_rows_workspace_size(c, batch, 64, max_kv, 8 * hkv)
+    one = -(-max_kv // 64) * 64 * hkv * hd * 4
+    parts = 296 * 2 * 128 * (hd * 4 + 8) + 296 * 64
+    assert min(one * batch, (1 << 30) - one) <= need <= max(1 << 30, one) + parts + 1024 * batch + 1024
