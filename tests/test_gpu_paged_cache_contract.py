@@ -1,6 +1,7 @@
-"""The paged-cache operators where the other tests of them do not go: values that are not
-finite, the cache's quantisation beside quantize()'s, and block tables far wider than the
-sequences."""
+"""The paged-cache operators against 64-bit forms where the other tests of them do not go:
+values that are not finite, the cache's quantisation beside quantize()'s, calls of nine to
+sixteen rows, every page size under the tensor-memory accelerator, batches of hundreds of
+sequences, and block tables far wider than the sequences."""
 import math
 
 import pytest
@@ -143,6 +144,60 @@ def test_append_beside_quantize(t, bits, hd, gs):
     room = step * (1.54 + 2 * n * 1.08 * P.U[t])
     bound = room[..., None] + P.U[t] * (va.abs() + vb.abs()) * 1.01
     assert bool(((va - vb).abs() <= bound).all())
+
+
+# ---------------------------------------------------------------------------- variants
+
+ROWS16 = [(14, 2, 128, [2, 1, 2, 0]), (8, 1, 128, [2, 2, 1, 1]), (10, 2, 128, [3, 1, 2, 3]),
+          (16, 4, 128, [4, 3, 0, 1]), (4, 4, 128, [16, 9, 1, 5]), (7, 1, 64, [2, 1, 0, 2]),
+          (8, 2, 64, [3, 4, 1, 2]), (3, 1, 64, [4, 5, 3, 1])]
+
+
+@pytest.mark.parametrize("t", [BF, HF])
+@pytest.mark.parametrize("bits,gs", base.CACHES)
+@pytest.mark.parametrize("hq,hkv,hd,news", [x for x in ROWS16])
+@pytest.mark.parametrize("how,page", [("tree", 16), ("prefill", 8), ("tree", 32)])
+def test_nine_to_sixteen_rows(t, bits, gs, hq, hkv, hd, news, how, page):
+    """A few new tokens over a quantised cache: sixteen rows of a kv head to a chunk."""
+    gs = min(gs, hd)
+    assert 8 < max(news) * (hq // hkv) <= 16
+    lens = [news[0] + 300, news[1], news[2] + 129, news[3] + 31]
+    p = base._problem(hq + gs + bits, t, bits, gs, hq, hkv, hd, page, lens, news,
+                      tree=how == "tree")
+    base._check(p, base._run(p, how))
+
+
+@pytest.mark.parametrize("bits,gs", [(4, 64), (8, 32)])
+def test_nine_to_sixteen_rows_split(bits, gs):
+    """The same over lengths that many CTAs share, and masks that are no tree."""
+    news, lens = [2, 2, 1], [9000, 2, 3001]
+    p = base._problem(81, BF, bits, gs, 28, 4, 128, 16, lens, news, tree=True)
+    base._check(p, base._run(p, "tree"))
+    p["masks"] = [2, 0, 0, 3, 0]
+    got = base._run(p, "tree")
+    assert not bool(got[2].any()) and bool(got[4].any())
+    base._check(p, got)
+
+
+@pytest.mark.parametrize("t", [BF, HF])
+@pytest.mark.parametrize("page", [8, 16, 32])
+@pytest.mark.parametrize("hq,hkv,hd", [(28, 4, 128), (8, 2, 64), (6, 2, 128), (5, 5, 64)])
+def test_tree_of_each_page_size(t, page, hq, hkv, hd):
+    """16-bit pages as boxes of 8, 16 and 32 rows; sequences that end at every place of a
+    page."""
+    news = [17, 40, 9, 64]
+    lens = [17 + 200, 40 + 23, 9 + 96, 64 + 1]
+    p = base._problem(page + hq, t, 16, 0, hq, hkv, hd, page, lens, news, tree=True)
+    base._check(p, base._run(p, "tree"))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_hundreds_of_trees(bits):
+    """More sequences than threads that count their tiles."""
+    news = [(7 * b) % 23 for b in range(300)]
+    lens = [n + (13 * b) % 90 for b, n in enumerate(news)]
+    p = base._problem(90, BF, bits, 64, 4, 1, 64, 16, lens, news, tree=True)
+    base._check(p, base._run(p, "tree"))
 
 
 # ---------------------------------------------------------------------------- wide tables
