@@ -1,14 +1,15 @@
 """The paged-cache operators against 64-bit forms where the other tests of them do not go:
 values that are not finite, the cache's quantisation beside quantize()'s, calls of nine to
 sixteen rows, every page size under the tensor-memory accelerator, batches of hundreds of
-sequences, and block tables far wider than the sequences."""
+sequences, block tables far wider than the sequences, and a model's attention layer over a
+quantised cache."""
 import math
 
 import pytest
 import torch
 
 import mlx_server_runtime_b200 as mxq
-from mlx_server_runtime_b200 import attention as A, qwen2
+from mlx_server_runtime_b200 import attention as A, core, qwen2
 
 import paged_util as P
 import test_gpu_paged_cache as base
@@ -249,3 +250,67 @@ def test_decoder_prefills_in_wide_tables():
         got.append(_peak(lambda: dec.prefill(ids, lengths)))
     assert torch.equal(got[1][0], got[2][0])
     assert abs(got[1][1] - got[2][1]) < 1 << 20
+
+
+# ---------------------------------------------------------------------------- in a model
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_attention_layer_over_a_quantised_cache(bits):
+    """The model's attention layer, head norms and all, prefills three prompts and takes a
+    decode step over a quantised cache. Its cache rows are the rule's on the rows the 16-bit
+    form writes, bit for bit; its output is o_proj of 64-bit attention over those rows.
+
+    The output may be off by what the attention may (carried through the weights' magnitudes),
+    by a weight's rounding to T (a half step of its largest term, code * scale or bias), by
+    32-bit sums over the inputs, and by its own rounding."""
+    cfg = qwen2.Qwen2Config(**base.CFG)
+    g = base._gen(17)
+    at = qwen2.Qwen2Attention(cfg, device="cuda", dtype=BF, generator=g, norm_jitter=0.1,
+                              bias_std=0.5)
+    hq, hkv, hd = at.n_heads, at.n_kv_heads, at.head_dim
+    cache = A.PagedKVCache(1, hkv, hd, 64, bits=bits)
+    plain = A.PagedKVCache(1, hkv, hd, 64)
+    k, v = cache.keys[0], cache.values[0]
+    kp, vp = plain.keys[0], plain.values[0]
+    bt = cache.allocate([200] * 3, generator=torch.Generator().manual_seed(5))
+    o = at.o_proj
+    W = mxq.dequantize(o.weight, o.scales, o.biases, o.group_size, o.bits).double()
+    per = 32 // o.bits
+    code = (o.weight.view(torch.int32).long().unsqueeze(-1) >>
+            (torch.arange(per, device="cuda") * o.bits)) & (2 ** o.bits - 1)
+    code = code.flatten(-2).unflatten(-1, (-1, o.group_size)).double()
+    terms = (code * o.scales.double().abs()[..., None] +
+             o.biases.double().abs()[..., None]).flatten(-2)
+    lens = [5, 37, 130]
+    for news in (lens, [1, 1, 1]):
+        if news is not lens:
+            lens = [n + 1 for n in lens]
+        at_pos = [range(L - n, L) for L, n in zip(lens, news)]
+        cu = [0] + [sum(news[:i + 1]) for i in range(3)]
+        batch = A.PagedBatch(bt, base._i32(lens), base._i32([p for r in at_pos for p in r]),
+                             cache.slots(bt, at_pos), max(lens),
+                             base._i32(cu) if max(news) > 1 else None, max(news))
+        x = base._randn(g, cu[-1], cfg.hidden_size).to(BF)
+        y = at(x, batch, k, v)
+        qkv = core.quantized_matmul(x, at.qkv_proj.weight, at.qkv_proj.scales, at.qkv_proj.biases,
+                                    True, cfg.group_size, cfg.bits, bias=at.qkv_proj.bias)
+        q = A.rope_kv_append(qkv, batch.positions, batch.slots, kp, vp, hq, hkv, hd, at.rope_base,
+                             at.q_norm, at.k_norm, at.eps)
+        held = cache.slots(bt, [range(L) for L in lens]).long()
+        kd, vd = A.kv_cache_read(k, v, held.int())
+        for got, rows in ((kd, kp), (vd, vp)):
+            w, s, b = P.quantized(rows.flatten(0, 1)[held], 64, bits)
+            ref = P.values(w, s, b, 64, bits).float().to(BF).cuda()
+            assert torch.equal(got, ref)
+        starts = [sum(lens[:i]) for i in range(3)]
+        parts = [P.attention(q[cu[i]:cu[i + 1]], [0, news[i]],
+                             kd[starts[i]:starts[i] + lens[i]].double(),
+                             vd[starts[i]:starts[i] + lens[i]].double(),
+                             {"page": lens[i], "pages": 1, "rows": [[0]]}, [lens[i]], at.scale,
+                             None, BF) for i in range(3)]
+        a, tol = (torch.cat(z).flatten(1) for z in zip(*parts))
+        ref = a @ W.T
+        top = a.abs() + tol
+        bound = tol @ W.abs().T + top @ terms.T * (P.U[BF] + (a.shape[1] + 16) * P.F)
+        bound = bound + P.U[BF] * (ref.abs() + bound)
+        assert bool(((y.double() - ref).abs() <= bound).all())
