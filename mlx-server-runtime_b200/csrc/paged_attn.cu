@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
             }
         }
 
-        uint32_t rows = row_id(t0, pid);
+        const uint32_t rows = row_id(t0, pid);
         bool mine_there = pid >= 0 && pid < c.pages;
         load_k(rows);
         load_v(rows);
@@ -372,7 +372,6 @@ __global__ void __launch_bounds__(ra::THREADS, ra::resident(HD, BITS, NT))
                 }
             }
             if (tile + 1 < te) load_v(next);
-            rows = next;
         }
 
         // Join the warps: (max, sum, O) of every row through shared memory.

@@ -38,24 +38,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, ui
         "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate));
 }
 
-// D (tensor memory) (+)= A (shared-memory descriptor) * B (shared-memory descriptor)
-__device__ __forceinline__ void umma_f16_ss(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
-                                            uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
-}
-
-// 8 consecutive 32-bit columns of this thread's tensor-memory lane
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-        : "memory");
-}
-
 // 16 consecutive 32-bit columns of this thread's tensor-memory lane
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
     asm volatile(
@@ -135,9 +117,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr));
     asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory");
 }
-// The same products and commit, executed by a converged warp: one thread of it (`leader`
-// nonzero) issues. Outside a branch of that thread's own, descriptors and addresses stay in
-// the warp's uniform registers.
+
+// Products and commit executed by a converged warp: one thread of it (`leader` nonzero)
+// issues. Outside a branch of that thread's own, descriptors and addresses stay in the warp's
+// uniform registers.
 __device__ __forceinline__ uint32_t elect_leader() {
     uint32_t r;
     asm volatile(
@@ -147,6 +130,7 @@ __device__ __forceinline__ uint32_t elect_leader() {
         : "=r"(r));
     return r;
 }
+// D (tensor memory) (+)= A (shared-memory descriptor) * B (shared-memory descriptor)
 __device__ __forceinline__ void umma_f16_ss_by(uint32_t leader, uint32_t tmem_d, uint64_t adesc,
                                                uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -156,6 +140,7 @@ __device__ __forceinline__ void umma_f16_ss_by(uint32_t leader, uint32_t tmem_d,
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader));
 }
+// D (tensor memory) (+)= A (tensor memory) * B (shared-memory descriptor)
 __device__ __forceinline__ void umma_f16_ts_by(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a,
                                                uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(

@@ -29,6 +29,15 @@ def test_no_read_only_loads(name):
     assert not re.search(r"\bconst\b[^;,(){}]*\*\s*__restrict__", s)
 
 
+@pytest.mark.parametrize("name", ["tcgen05.cuh", "kv_dequant.cuh", "rows_units.cuh",
+                                  "quant_rule.cuh", "overlap.cuh"])
+def test_every_helper_has_a_caller(name):
+    all_of_it = "".join(source(f) for f in sorted(os.listdir(CSRC)))
+    helpers = set(re.findall(r"__forceinline__[\w:&* ]*?(\w+)\(", source(name)))
+    assert helpers
+    assert [h for h in sorted(helpers) if len(re.findall(rf"\b{h}\b", all_of_it)) < 2] == []
+
+
 def test_prefill_bounds_its_lengths():
     """max_kv_len is at most what the block table holds (two pages of 16 here)."""
     c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
