@@ -38,6 +38,18 @@ def test_every_helper_has_a_caller(name):
     assert [h for h in sorted(helpers) if len(re.findall(rf"\b{h}\b", all_of_it)) < 2] == []
 
 
+def test_tensor_memory_loads_are_waited_for():
+    """Registers that a tcgen05.ld fills may be used after its wait. Only what one asm statement
+    holds, or what passes through a statement behind the wait, is sure to stay in that order."""
+    loads = [f for f in re.split(r"(?=__device__ __forceinline__)", source("tcgen05.cuh"))
+             if "tcgen05.ld." in f]
+    assert loads
+    for f in loads:
+        statement = f.split("tcgen05.ld.")[-1].split(");")[0]
+        tied = re.search(r'wait::ld.*asm volatile\("" : "\+r"', f, flags=re.S)
+        assert tied or "tcgen05.wait::ld" in statement, f[:80]
+
+
 def test_prefill_bounds_its_lengths():
     """max_kv_len is at most what the block table holds (two pages of 16 here)."""
     c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
