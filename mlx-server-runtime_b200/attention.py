@@ -190,7 +190,9 @@ def rope_kv_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tens
     k_cache / v_cache [pages, page_size, n_kv_heads, head_dim], or quantized into a pair
     of QuantizedKV. With q_norm / k_norm [head_dim] each query / key head is RMS-normed
     first (the head norms of Qwen3-style attention, models/qwen3.py of the reference),
-    in the same launch and with one rounding. A group of a QuantizedKV row that would hold a
+    in the same launch and with one rounding; angles are then, and into a QuantizedKV, reduced
+    in 64 bits, where the plain form into 16-bit caches takes them in 32 (off by some 2^-23 of
+    the angle, 10^-2 rad at position 10^5). A group of a QuantizedKV row that would hold a
     NaN or an infinity stands for NaN as a whole. Returns the rotated queries
     [T, n_heads, head_dim]. Two tokens of a call must not share a slot."""
     if q_norm is not None or k_norm is not None or isinstance(k_cache, QuantizedKV) or \

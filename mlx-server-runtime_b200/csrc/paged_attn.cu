@@ -19,17 +19,19 @@
 //   S^T = K Q^T    A = 16 keys x 16 dims, straight from global memory: a lane's dims are
 //                  contiguous in its key's row, and q is permuted to match once
 //   O^T = V^T P^T  A = 16 dims x 16 keys, pairs of keys joined by byte permutes; P^T is S^T
-//                  rounded to T and transposed in registers (movmatrix)
+//                  rounded to T (a 16-bit product's operand: half a step each, 2.0e-3 to
+//                  2.3e-3 of a bf16 result where unrounded ones leave 1.7e-3, the result's own
+//                  rounding) and transposed in registers (movmatrix)
 // so packed codes go from their load through registers into the product; shared memory
 // holds only the four warps' results at the end of an item. Rows are loaded into registers a
 // tile ahead, page ids two.
 //
 // What bounds it is how rows arrive: 32 sequences of up to 16384 4-bit keys (4 kv heads of 128,
-// 196 MB, 16384 down to 4500 keys) take 80 us, 2.4 TB/s, of which 15 do not depend on the
+// 192 MB, 16384 down to 4500 keys) take 80 us, 2.4 TB/s, of which 15 do not depend on the
 // lengths; with the loads left out they take 47, with the unpacking left out 74, and with
 // keys that fit L2 the rate is the same. Sixteen-key pages of one head are 64-byte pieces, and
-// a head's scales a quarter of their sectors. 8-bit codes of the same heads move 2.9 TB/s,
-// 16-bit rows 4.2. Shorter runs (94 to 115 us) were slower, as were four heads' warps in one
+// a head's scales a quarter of their sectors. 8-bit codes of the same heads move 3.5 TB/s,
+// 16-bit rows 4.7. Shorter runs (94 to 115 us) were slower, as were four heads' warps in one
 // CTA, which share those sectors but join four times the parts (75 us here, but 32 for 23 with
 // 64 sequences of 1000 keys and 89 for 82 over 16 bits).
 #include "common.cuh"
@@ -75,8 +77,9 @@ __device__ __forceinline__ void ldw(const void* at, uint32_t (&r)[N]) {
 }
 
 // CTAs of an SM: what the registers of a variant allow (and the launch bounds ask for).
-// Three rather than four for 4 bits and heads of 128, which spills nothing: 32 sequences of
-// up to 16384 keys 80 us (four: 78), one of 32768 19 (22), 64 of 1000 24 (29).
+// Three rather than four for heads of 128, which spills nothing: 32 sequences of up to 16384
+// 4-bit keys 80 us (four: 78), 64 of 1000 22.7 (23.7), 16 of 4097 20.7 (21.2), and over 8 bits
+// 32 of up to 16384 105 (130).
 constexpr int resident(int hd, int bits, int nt) {
     return nt == 2 ? 2 : bits == 16 ? (hd == 64 ? 3 : 2) : hd == 64 ? 4 : 3;
 }
@@ -526,9 +529,11 @@ namespace {
 
 // How a call is run: eight rows to a chunk where a decode step's heads fit them; sixteen
 // of a quantised cache; and from then on up to 128, whole tokens of them, as the M rows of
-// tcgen05 products. (Eight sequences of 4096 keys, seven heads to a kv head: two tokens over
-// 4 bits 23 us with sixteen rows to a chunk and 36 as M rows, whose keys are expanded first;
-// over 16 bits 33 and 26.)
+// tcgen05 products. The kernel of few rows takes one chunk a sequence. Nine to sixteen rows
+// over 4 bits, 28/4 heads of 128, with sixteen rows to a chunk and as M rows, whose keys are
+// expanded first: one sequence of 512 keys 11.7 and 14.6 us, of 16384 19.5 and 38; eight of 1024
+// 14.6 and 24.5, of 4096 22 and 36, of 16384 40 and 94; 32 of 4096 41 and 90. Over 8 bits the
+// same within a fifth. Over 16 bits, where nothing is expanded, eight of 4096 take 33 and 26.
 struct Plan {
     bool tc;
     int rows, kt, parts, group;
@@ -551,7 +556,7 @@ Plan plan_of(const KvCache& c, const RowsArgs& a) {
     long long units = tiles * (p.tc ? c.Hkv * (p.group > 1 ? 1 : chunks) : 1);  // of a sequence
     long long groups = most / p.group > 1 ? most / p.group : 1;
     // runs of fewer than four tiles cost more to join than they save: two CTAs an SM then
-    // (a sequence of 32768 4-bit keys 17 us, with three 19; 16 of 4097 17 and 19)
+    // (a sequence of 32768 4-bit keys 18 us, with three 19; 16 of 4097 8-bit ones 17.6 and 19)
     const long long few = 296 / p.group;
     if (!p.tc && units * a.batch < 4 * groups && few < groups) groups = few > 1 ? few : 1;
     if (units < groups && units * a.batch < groups) groups = units * a.batch > 1 ? units * a.batch : 1;

@@ -10,7 +10,8 @@
 //   softmax     thread = row: S is read back, P = exp2(S * scale - m) goes back into the
 //               columns of S as 16-bit pairs. m follows the running maximum only when a
 //               score passes it by 2^8, so O is rescaled seldom; P then reaches 256, which
-//               costs neither type precision.
+//               costs neither type precision. (Rounded to T as a 16-bit product's operand: half
+//               a step each, 2.0e-3 to 2.3e-3 of a bf16 result where unrounded ones leave 1.7e-3.)
 //   O += P V    M = 128, N = head size, K = 64: P read from tensor memory, V from shared
 //               memory as it lies (key rows, dimensions contiguous)
 // S, K and V have two buffers each, so S of the next tile is there when the softmax of this
@@ -19,8 +20,9 @@
 // box to a page and 64 dims (one warp for both takes 2100 cycles a tile of 16-key pages,
 // longer than the softmax); warp 5 issues the products. A chunk is whole tokens, 128 / G of
 // them, so that its queries are one box too (64 dims, G heads, the tokens): loaded by a
-// warp's lanes they took 5000 cycles of every item. Two CTAs share an SM (96 KB of shared
-// memory and 256 columns each).
+// warp's lanes they took 5000 cycles of every item. Two CTAs share an SM: 105 KB of dynamic
+// shared memory (heads of 128) and 256 of the 512 columns each. For heads of 64 it is registers,
+// 128 a thread, that leave no room for a third, which would wait for columns.
 // Work is shared out as in rows_units.cuh. Every wait is bounded: on a timeout the CTA
 // records an error, its roles stop, what is in flight is waited for, tensor memory is
 // freed and the kernel returns.

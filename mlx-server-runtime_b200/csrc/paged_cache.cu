@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(128) norm_rope_append_kernel(const __grid_cons
             }
         } else if (__any_sync(0xffffffffu, put)) {
             // (a warp of query heads is done: quantising them all the same took 117 us where
-            // the 16-bit append of 8190 tokens takes 43.) Every lane takes part in the
+            // the 16-bit append of 8190 tokens takes 34.) Every lane takes part in the
             // shuffles; lanes of a query head store nothing.
             const float p[4] = {Elem<T>::lo(lo.x), Elem<T>::hi(lo.x), Elem<T>::lo(lo.y),
                                 Elem<T>::hi(lo.y)};
