@@ -346,11 +346,15 @@ __global__ void __launch_bounds__(rt::THREADS, 2)
         while (more || npv < ns) {
             // S runs up to two tiles ahead of P V. An item's first waits for its queries, and
             // they for the last S of the item before: P V goes first then.
+            // (One poll's answer is each lane's own: they vote on it, and lanes that left a wait
+            // early are waited for, or some could fall behind by the two phases a barrier holds.)
+            __syncwarp();
             const bool begin = tile == w.t0;
             const uint32_t sb = ns & 1, vb = npv & 1;
             if (more && ns - npv < 2 &&
                 (!begin || npv == ns ||
-                 (mbar_try_wait(smem_u32(&q_full), nq & 1) && mbar_try_wait(smem_u32(k_full + sb), ns >> 1 & 1)))) {
+                 __all_sync(0xffffffffu, mbar_try_wait(smem_u32(&q_full), nq & 1) &&
+                                             mbar_try_wait(smem_u32(k_full + sb), ns >> 1 & 1)))) {
                 if ((begin && !spin(&q_full, nq++)) || !spin(k_full + sb, ns >> 1)) break;
                 tc_fence_after();
                 const uint32_t bit = 1u << (ns & 31);

@@ -71,3 +71,14 @@ def test_expansion_workspace_is_bounded(batch, max_kv, hkv, hd):
     one = -(-max_kv // 64) * 64 * hkv * hd * 4
     parts = 296 * 2 * 128 * (hd * 4 + 8) + 296 * 64
     assert min(one * batch, (1 << 30) - one) <= need <= max(1 << 30, one) + parts + 1024 * batch + 1024
+
+
+def test_the_warp_that_issues_products_decides_as_one():
+    """Its lanes poll barriers each for itself. What it does next follows from a vote, and each
+    round begins with all lanes there: a lane left two phases behind would wait for good."""
+    s = source("paged_attn_tc.cu")
+    role = s[s.index("else if (warp == WARP_MMA)"):]
+    loop = role[role.index("while (more || npv < ns)"):role.index("umma_commit_by(leader, smem_u32(&drained))")]
+    assert re.match(r"[^;]*\{\s*__syncwarp\(\);", loop)
+    voted = "".join(re.findall(r"__all_sync\(0xffffffffu,.*?\)\)\s*\{", loop, flags=re.S))
+    assert voted.count("mbar_try_wait(") == loop.count("mbar_try_wait(") > 0
